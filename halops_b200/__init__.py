@@ -5,23 +5,43 @@ Drop-in for the reference's ``halops.group_wise_quant``, ``halops.dense_gemm``,
 ``halops.low_latency_mma_gemm`` and ``halops.rms_norm_quant`` (plus ``interleave_gate_up`` and ``EpilogueOp``): same
 Python signatures, executed by hand-written CUDA/PTX kernels through a C-ABI
 shared library.  There is no CPU path and no fallback.
+
+Beside them, without a counterpart in the reference: FP8 products with a float32 scale per block of 128
+(``block_quant``, ``swiglu_block_quant``, ``block_gemm``, ``group_block_gemm``) and tokens in the order of their experts and
+back, with gradients (``moe_sort``, ``moe_permute``, ``moe_permute_block_quant``, ``moe_unpermute``, ``moe_permute_backward``,
+``moe_unpermute_backward``).
 """
 
 from .gemm import (
     EpilogueOp,
     batch_gemm,
+    block_gemm,
+    block_quant,
     dense_gemm,
+    group_block_gemm,
     group_contiguous_gemm,
     group_masked_gemm,
     group_wise_quant,
     interleave_gate_up,
     low_latency_mma_gemm,
     rms_norm_quant,
+    swiglu_block_quant,
+)
+from .moe import (
+    MoeSort,
+    moe_permute,
+    moe_permute_backward,
+    moe_permute_block_quant,
+    moe_sort,
+    moe_unpermute,
+    moe_unpermute_backward,
 )
 from ._native import lib_path
 
-__all__ = ["EpilogueOp", "batch_gemm", "dense_gemm", "group_contiguous_gemm", "group_masked_gemm",
-           "group_wise_quant", "interleave_gate_up", "low_latency_mma_gemm", "rms_norm_quant", "device_status", "selftest_bounded_wait", "describe_tile",
+__all__ = ["EpilogueOp", "MoeSort", "batch_gemm", "block_gemm", "block_quant", "dense_gemm", "group_block_gemm",
+           "group_contiguous_gemm", "group_masked_gemm", "group_wise_quant", "interleave_gate_up", "low_latency_mma_gemm",
+           "moe_permute", "moe_permute_backward", "moe_permute_block_quant", "moe_sort", "moe_unpermute",
+           "moe_unpermute_backward", "rms_norm_quant", "swiglu_block_quant", "device_status", "selftest_bounded_wait", "describe_tile",
            "describe_group_tile", "lib_path"]
 __version__ = "0.1.0"
 

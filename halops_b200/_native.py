@@ -55,6 +55,25 @@ SIGNATURES = {
                                                              c_size_t]),
     "hq_describe_group_tile": (c_int, [c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_int, c_int, c_int, c_char_p,
                                        c_size_t]),
+    "hq_block_quant": (c_int, [c_void_p, c_i64, c_i64, c_int, c_i64, c_i64, c_i64, c_int, c_int, c_int, c_void_p, c_void_p,
+                               c_int, c_void_p, c_char_p, c_size_t]),
+    "hq_swiglu_block_quant": (c_int, [c_void_p, c_i64, c_int, c_i64, c_i64, c_void_p, c_int, c_void_p, c_void_p, c_int,
+                                      c_void_p, c_char_p, c_size_t]),
+    "hq_block_gemm": (c_int, [c_void_p] * 5 + [c_int, c_i64, c_i64, c_i64, c_int, c_i64, c_int, c_int, c_int, c_void_p,
+                                               c_char_p, c_size_t]),
+    "hq_group_block_gemm": (c_int, [c_void_p] * 6 + [c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_int, c_int, c_int,
+                                                     c_void_p, c_char_p, c_size_t]),
+    "hq_moe_sort": (c_int, [c_void_p, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                            c_int, c_void_p, c_char_p, c_size_t]),
+    "hq_moe_permute": (c_int, [c_void_p, c_i64, c_i64, c_i64, c_i64, c_void_p, c_void_p, c_void_p, c_i64, c_i64, c_int, c_int,
+                               c_void_p, c_int, c_void_p, c_char_p, c_size_t]),
+    "hq_moe_permute_block_quant": (c_int, [c_void_p, c_i64, c_int, c_i64, c_i64, c_i64, c_void_p, c_void_p, c_void_p, c_i64,
+                                           c_i64, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_char_p, c_size_t]),
+    "hq_moe_unpermute": (c_int, [c_void_p, c_i64, c_int, c_i64, c_i64, c_i64, c_i64, c_void_p, c_void_p, c_int, c_void_p,
+                                 c_int, c_void_p, c_char_p, c_size_t]),
+    "hq_moe_unpermute_backward": (c_int, [c_void_p, c_i64, c_void_p, c_i64, c_int, c_i64, c_i64, c_i64, c_i64, c_void_p,
+                                          c_void_p, c_void_p, c_i64, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int,
+                                          c_void_p, c_char_p, c_size_t]),
     "hq_sm_count": (c_int, [c_int]),
     "hq_hold_switches": (None, [c_int]),
     "hq_device_status": (c_int, [c_int, c_void_p, ctypes.POINTER(ctypes.c_uint32), c_char_p, c_size_t]),
@@ -103,6 +122,8 @@ class _NoFastPath:
         return None
 
     group_wise_quant = rms_norm_quant = dense_gemm = grouped_gemm = _none
+    block_quant = swiglu_block_quant = block_gemm = _none
+    moe_sort = moe_permute = moe_permute_block_quant = moe_unpermute = moe_unpermute_backward = _none
 
 
 # The module of csrc/fast_path.cpp, which makes the ordinary call of an entry point natively; None until
@@ -120,6 +141,9 @@ def _import_fast_path(handle):
     module.bind(*(ctypes.cast(getattr(handle, name), c_void_p).value for name in (
         "hq_group_wise_quant", "hq_rms_norm_quant", "hq_dense_gemm", "hq_dense_gemm_situ_quant",
         "hq_describe_group_tile", "hq_group_masked_gemm", "hq_group_contiguous_gemm", "hq_hold_switches")))
+    module.bind_block(*(ctypes.cast(getattr(handle, name), c_void_p).value for name in (
+        "hq_block_quant", "hq_swiglu_block_quant", "hq_block_gemm", "hq_group_block_gemm", "hq_moe_sort", "hq_moe_permute",
+        "hq_moe_permute_block_quant", "hq_moe_unpermute", "hq_moe_unpermute_backward")))
     return module
 
 

@@ -15,10 +15,10 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libhalops_b200.so")
-SOURCES = ("quant.cu", "gemm.cu")
+SOURCES = ("quant.cu", "gemm.cu", "block_quant.cu", "block_gemm.cu", "moe.cu")
 ABI_HEADER = os.path.join(PKG, "..", "include", "halops_b200.h")
 FAST_PATH_DEPS = (os.path.join(CSRC, "fast_path.cpp"), ABI_HEADER)
-HEADERS = ("common.cuh", "ptx.cuh", "decode.cuh")
+HEADERS = ("common.cuh", "gemm_common.cuh", "ptx.cuh", "decode.cuh", "block_quant.cuh")
 
 
 try:
@@ -93,6 +93,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
             "-O3", "-std=c++17", "-lineinfo",
             "-Xcompiler", "-fPIC",
             "-shared",
+            "--threads", "0",
             "-o", LIB_PATH,
         ]
         if verbose:

@@ -1,0 +1,736 @@
+// FP8 products whose operands carry a float32 scale per block of 128 along K:
+//
+//   out[m, n] = sum over blocks b of sfa[m, b] * sfb[n / 128 or n, b] * sum over k in b of a[m, k] * w[n, k]
+//
+// dense, or with the rows of `a` in runs of one expert each.  The tensor cores' block scales are powers of two per 32 values,
+// so a float32 scale cannot ride along with the MMA: the products of one block of 128 are summed in tensor memory (four MMAs,
+// K = 32 each), and the sums then leave for registers, where they are scaled and added up in float32.
+//
+// Per CTA (one per SM, persistent over output tiles of 128 x BN):
+//   warps 0-7  promotion: tcgen05.ld of a block's sums, accumulators += scale * sums (two columns an instruction); after the last
+//              block the accumulators are rounded once and stored.  A thread has one row and half of the tile's columns.
+//   warp 8     TMA producer: A and B tiles (128-byte swizzle) into a ring of stages
+//   warp 9     issues the MMAs of a block into the next of 2 (BN = 256) or 4 buffers of tensor memory
+//   warp 10    (a scale per row of the second operand) brings the scales of a block into shared memory
+//
+// Every mbarrier wait is bounded, as in the other GEMM kernels: a role that waits longer than kTimeoutNs records a code in the
+// status word, raises the CTA's abort flag and all roles leave through the common teardown.
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "gemm_common.cuh"
+#include "ptx.cuh"
+
+namespace hq {
+namespace {
+
+constexpr int kTileM = 128;
+constexpr int kBlockK = 128;  // values, and bytes, of a k-tile row
+constexpr int kPromoWarps = 8;
+constexpr int kMaxExperts = 1024;
+constexpr int kSmemBudget = 232448;
+constexpr int kScaleSlots = 4;
+
+struct BlockBars {
+    uint64_t full[8];
+    uint64_t empty[8];
+    uint64_t acc_full[4];
+    uint64_t acc_empty[4];
+    uint64_t sf_full[kScaleSlots];
+    uint64_t sf_empty[kScaleSlots];
+    uint32_t tmem_base;
+    uint32_t abort;
+};
+
+template <int BN, bool kRowScales>
+struct BlockCfg {
+    static constexpr int kABytes = kTileM * kBlockK;
+    static constexpr int kBBytes = BN * kBlockK;
+    static constexpr int kStageBytes = kABytes + kBBytes;
+    static constexpr int kBarBytes = 512;
+    static constexpr int kTableBytes = (kMaxExperts + 8) * 8;                // grouped: row tiles before, first row of, each expert
+    static constexpr int kScaleBytes = kRowScales ? kScaleSlots * BN * 4 : 0;
+    static constexpr int kExtra = kBarBytes + kTableBytes + kScaleBytes + 1024;
+    static constexpr int kFit = (kSmemBudget - kExtra) / kStageBytes;
+    static constexpr int kStages = kFit > 8 ? 8 : kFit;
+    static constexpr int kSmemBytes = kStages * kStageBytes + kExtra;
+    static constexpr int kBufs = BN == 256 ? 2 : 4;
+    static constexpr int kTmemCols = kBufs * BN;
+    static constexpr int kCols = BN / 2;  // columns of a promotion warp
+    // BN = 256: 128 accumulators a thread; the third warpgroup gives registers to the other two (168 * 384 = 232 * 256 + 40 * 128)
+    static constexpr bool kRegSplit = BN == 256;
+    static constexpr int kThreads = kRegSplit ? 384 : (kPromoWarps + 2 + (kRowScales ? 1 : 0)) * 32;
+    static_assert(sizeof(BlockBars) <= kBarBytes && kStages >= 3 && kTmemCols <= 512, "budgets");
+    static_assert(kTileM * (BN + 4) * 4 <= kStages * kStageBytes, "split-K partial sums fit into the ring");
+};
+
+struct BlockArgs {
+    const float* sfa;
+    const float* sfb;
+    void* out;
+    const int* offsets;  // grouped: first row of each expert, and the end of the last
+    int64_t ldo;
+    int m, n, k_tiles, tiles_m, tiles_n;
+    int n_blocks;   // scales of the second operand per expert along N (rows of sfb)
+    int experts;
+    int box_rows;   // rows of `a` per copy
+    int out_type;   // HQ_DTYPE_*
+    int out_align;  // 32, 16 or less: bytes that every row of the output starts on
+    int split;      // CTAs of a cluster that share a tile's k-tiles
+    int pdl;
+};
+
+struct BlockTile {
+    int row0, valid, n0, expert;
+};
+
+// The sequence of a CTA's tiles; every role walks it for itself.
+template <int BN, bool kGrouped>
+struct BlockWalk {
+    const BlockArgs& p;
+    const int* const tiles_before;  // grouped, in shared memory: [experts + 1]
+    const int* const first_row;
+    int tile;
+    const int step, total;
+    __device__ __forceinline__ BlockWalk(const BlockArgs& args, const int* tables, int first, int step_)
+        : p(args), tiles_before(tables), first_row(tables + kMaxExperts + 8), tile(first), step(step_),
+          total(kGrouped ? tables[args.experts] * args.tiles_n : args.tiles_m * args.tiles_n) {}
+    __device__ __forceinline__ bool next(BlockTile& t) {
+        if (tile >= total) return false;
+        if constexpr (kGrouped) {
+            // the expert whose tiles hold this one
+            int lo = 0, hi = p.experts;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (tiles_before[mid] * p.tiles_n <= tile) lo = mid; else hi = mid;
+            }
+            // within an expert down the rows first: the CTAs that run at the same time share the weight's tiles
+            const int row_tiles = tiles_before[lo + 1] - tiles_before[lo];
+            const int r = tile - tiles_before[lo] * p.tiles_n;
+            const int n_tile = r / row_tiles;
+            t.expert = lo;
+            t.row0 = first_row[lo] + (r - n_tile * row_tiles) * kTileM;
+            t.valid = min(kTileM, first_row[lo + 1] - t.row0);
+            t.n0 = n_tile * BN;
+        } else {
+            // groups of 8 row tiles, then across the columns: one wave of CTAs shares a small set of tiles in L2
+            constexpr int kGroup = 8;
+            const int per = kGroup * p.tiles_n;
+            const int g = tile / per, first_m = g * kGroup;
+            const int gsz = min(kGroup, p.tiles_m - first_m);
+            const int r = tile - g * per;
+            const int n_tile = r / gsz;
+            t.expert = 0;
+            t.row0 = (first_m + r - n_tile * gsz) * kTileM;
+            t.valid = min(kTileM, p.m - t.row0);
+            t.n0 = n_tile * BN;
+        }
+        tile += step;
+        return true;
+    }
+};
+
+// d (+)= a . b^T, K = 32 e4m3 values, float32 sums in tensor memory.
+__device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+        "}" ::"r"(d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// 32 lanes x 16 columns; the values are there behind load_wait on the same registers.
+__device__ __forceinline__ void load_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void load_wait(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t pack16(float lo, float hi, int type) {
+    uint32_t r;
+    if (type == HQ_DTYPE_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        memcpy(&r, &h, 4);
+    } else {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        memcpy(&r, &h, 4);
+    }
+    return r;
+}
+
+__device__ __forceinline__ void store_32_bytes(void* p, const uint32_t (&w)[8], int align) {
+    if (align >= 32) {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                     "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                     : "memory");
+    } else {
+        reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+}
+
+// kN neighbouring values of a row from column `col` on, `left` of which exist.
+template <int kN>
+__device__ __forceinline__ void store_values(const float (&f)[kN], void* out, int64_t at, int left, int type, int align) {
+    if (type == HQ_DTYPE_FP32) {
+        float* const o = static_cast<float*>(out) + at;
+        if (left >= kN && align >= 16) {
+#pragma unroll
+            for (int i = 0; i < kN; i += 4) *reinterpret_cast<float4*>(o + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+                if (i < left) o[i] = f[i];
+            }
+        }
+        return;
+    }
+    uint32_t w[kN / 2];
+#pragma unroll
+    for (int i = 0; i < kN / 2; ++i) w[i] = pack16(f[2 * i], f[2 * i + 1], type);
+    uint16_t* const o = static_cast<uint16_t*>(out) + at;
+    if (left >= kN && align >= 16) {
+        if constexpr (kN == 16) {
+            store_32_bytes(o, w, align);
+        } else {
+            *reinterpret_cast<uint2*>(o) = make_uint2(w[0], w[1]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            if (i < left) o[i] = uint16_t(w[i / 2] >> (i % 2 * 16));
+        }
+    }
+}
+
+template <int BN, bool kRowScales, bool kGrouped, bool kSplit>
+__global__ void __launch_bounds__((BlockCfg<BN, kRowScales>::kThreads), 1)
+block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ BlockArgs p) {
+    using C = BlockCfg<BN, kRowScales>;
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t a_base = ptx::smem_u32(smem);
+    const uint32_t b_base = a_base + C::kStages * C::kABytes;
+    constexpr int kBarOffset = C::kStages * C::kStageBytes;
+    BlockBars* const bars = reinterpret_cast<BlockBars*>(smem + kBarOffset);
+    int* const tables = reinterpret_cast<int*>(smem + kBarOffset + C::kBarBytes);
+    float* const scales = reinterpret_cast<float*>(smem + kBarOffset + C::kBarBytes + C::kTableBytes);
+    volatile uint32_t* const abort = &bars->abort;
+    const int warp = warp_index();
+    const int lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::kStages; ++s) {
+            ptx::mbar_init(ptx::smem_u32(&bars->full[s]), 1);
+            ptx::mbar_init(ptx::smem_u32(&bars->empty[s]), 1);
+        }
+        for (int s = 0; s < C::kBufs; ++s) {
+            ptx::mbar_init(ptx::smem_u32(&bars->acc_full[s]), 1);
+            ptx::mbar_init(ptx::smem_u32(&bars->acc_empty[s]), kPromoWarps);
+        }
+        for (int s = 0; s < kScaleSlots; ++s) {
+            ptx::mbar_init(ptx::smem_u32(&bars->sf_full[s]), 1);
+            ptx::mbar_init(ptx::smem_u32(&bars->sf_empty[s]), kPromoWarps);
+        }
+        bars->abort = 0;
+        ptx::fence_mbar_init();
+        ptx::prefetch_tmap(&tm_a);
+        ptx::prefetch_tmap(&tm_b);
+    }
+    if (warp == 9) {
+        ptx::tmem_alloc<1>(ptx::smem_u32(&bars->tmem_base), C::kTmemCols);
+        ptx::tmem_relinquish<1>();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = bars->tmem_base;
+
+    // nothing below may run before the preceding kernel's writes are visible
+    ptx::pdl_wait();
+    if constexpr (kGrouped) {
+        if (warp == 0) {
+            // row tiles before each expert; offsets that go back or point outside are clamped, so that no row is touched that is not there
+            int before = 0, last = 0;
+            int* const first_row = tables + kMaxExperts + 8;
+            for (int e0 = 0; e0 <= p.experts; e0 += 32) {
+                const int e = e0 + lane;
+                int start = e <= p.experts ? min(max(__ldg(p.offsets + e), 0), p.m) : 0;
+#pragma unroll
+                for (int d = 1; d < 32; d *= 2) {
+                    const int v = __shfl_up_sync(0xffffffffu, start, d);
+                    if (lane >= d) start = max(start, v);
+                }
+                start = max(start, last);
+                int prev = __shfl_up_sync(0xffffffffu, start, 1);
+                if (lane == 0) prev = last;
+                // tiles of expert e - 1
+                int sum = e >= 1 && e <= p.experts ? (start - prev + kTileM - 1) / kTileM : 0;
+#pragma unroll
+                for (int d = 1; d < 32; d *= 2) {
+                    const int v = __shfl_up_sync(0xffffffffu, sum, d);
+                    if (lane >= d) sum += v;
+                }
+                if (e <= p.experts) {
+                    first_row[e] = start;
+                    tables[e] = before + sum;
+                }
+                before += __shfl_sync(0xffffffffu, sum, 31);
+                last = __shfl_sync(0xffffffffu, start, 31);
+            }
+        }
+        __syncthreads();
+    }
+    const int rank = kSplit ? int(blockIdx.x) % p.split : 0;
+    const int first = kSplit ? int(blockIdx.x) / p.split : int(blockIdx.x);
+    const int step = kSplit ? int(gridDim.x) / p.split : int(gridDim.x);
+    const int k_begin = kSplit ? int(int64_t(p.k_tiles) * rank / p.split) : 0;
+    const int k_end = kSplit ? int(int64_t(p.k_tiles) * (rank + 1) / p.split) : p.k_tiles;
+
+    if (warp >= kPromoWarps) {
+    if constexpr (C::kRegSplit) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 8) {
+        // ------------------------------------------------------------ TMA producer
+        uint32_t it = 0;
+        bool ok = true;
+        BlockWalk<BN, kGrouped> walk(p, tables, first, step);
+        BlockTile t;
+        while (ok && walk.next(t)) {
+            const int boxes = (t.valid + p.box_rows - 1) / p.box_rows;
+            const int b_row = t.expert * p.n + t.n0;
+            const uint32_t bytes = uint32_t(boxes * p.box_rows * kBlockK + C::kBBytes);
+            for (int kt = k_begin; kt < k_end; ++kt, ++it) {
+                const uint32_t s = it % C::kStages;
+                ok = wait_bar<true>(ptx::smem_u32(&bars->empty[s]), ((it / C::kStages) & 1u) ^ 1u, abort, kStatusProducer);
+                if (!ok) break;
+                const uint32_t full = ptx::smem_u32(&bars->full[s]);
+                if (ptx::elect_one()) ptx::mbar_arrive_expect_tx(full, bytes);
+                if (ptx::elect_one()) ptx::tma_load_2d(b_base + s * C::kBBytes, &tm_b, kt * kBlockK, b_row, full);
+                for (int b = 0; b < boxes; ++b) {
+                    if (ptx::elect_one()) {
+                        ptx::tma_load_2d(a_base + s * C::kABytes + b * p.box_rows * kBlockK, &tm_a, kt * kBlockK, t.row0 + b * p.box_rows, full);
+                    }
+                }
+            }
+        }
+        ptx::pdl_launch_dependents();
+    } else if (warp == 9) {
+        // ------------------------------------------------------------ MMA issuer
+        // float32 sums, e4m3 operands, both K-major; N >> 3, M >> 4
+        constexpr uint32_t idesc = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(kTileM >> 4) << 24);
+        uint32_t it = 0;
+        bool ok = true;
+        BlockWalk<BN, kGrouped> walk(p, tables, first, step);
+        BlockTile t;
+        while (ok && walk.next(t)) {
+            for (int kt = k_begin; kt < k_end; ++kt, ++it) {
+                const uint32_t s = it % C::kStages, buf = it % C::kBufs;
+                ok = wait_bars<true>(ptx::smem_u32(&bars->full[s]), (it / C::kStages) & 1u, true, ptx::smem_u32(&bars->acc_empty[buf]),
+                               ((it / C::kBufs) & 1u) ^ 1u, abort, kStatusMma);
+                if (!ok) break;
+                ptx::tc_fence_after();
+                const uint64_t adesc = ptx::smem_desc(a_base + s * C::kABytes, 16, 1024, 2);
+                const uint64_t bdesc = ptx::smem_desc(b_base + s * C::kBBytes, 16, 1024, 2);
+                const uint32_t d = tmem + buf * BN;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    // K = 32 bytes: the start address moves inside of the 128-byte swizzle atom
+                    if (ptx::elect_one()) mma_e4m3(d, adesc + 2 * j, bdesc + 2 * j, idesc, j > 0 ? 1u : 0u);
+                }
+                if (ptx::elect_one()) ptx::tc_commit(ptx::smem_u32(&bars->acc_full[buf]));
+                if (ptx::elect_one()) ptx::tc_commit(ptx::smem_u32(&bars->empty[s]));
+            }
+        }
+    } else if (kRowScales && warp == 10) {
+        // ------------------------------------------------------------ scales of the second operand's rows
+        // four k-tiles are in registers before the slots are free
+        uint32_t it = 0;
+        bool ok = true;
+        BlockWalk<BN, kGrouped> walk(p, tables, first, step);
+        BlockTile t;
+        while (ok && walk.next(t)) {
+            for (int k0 = k_begin; ok && k0 < k_end; k0 += kScaleSlots) {
+                float v[kScaleSlots][BN / 32];
+#pragma unroll
+                for (int i = 0; i < kScaleSlots; ++i) {
+#pragma unroll
+                    for (int j = 0; j < BN / 32; ++j) {
+                        const int n = t.n0 + j * 32 + lane;
+                        v[i][j] = k0 + i < k_end && n < p.n ? __ldg(p.sfb + (int64_t(t.expert) * p.n + n) * p.k_tiles + k0 + i) : 0.0f;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kScaleSlots; ++i) {
+                    if (k0 + i >= k_end) break;
+                    const uint32_t slot = it % kScaleSlots;
+                    ok = wait_bar<true>(ptx::smem_u32(&bars->sf_empty[slot]), ((it / kScaleSlots) & 1u) ^ 1u, abort, kStatusProducer);
+                    if (!ok) break;
+#pragma unroll
+                    for (int j = 0; j < BN / 32; ++j) scales[slot * BN + j * 32 + lane] = v[i][j];
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&bars->sf_full[slot]));
+                    ++it;
+                }
+            }
+        }
+    }
+    } else {
+        // ------------------------------------------------------------ promotion and epilogue
+        if constexpr (C::kRegSplit) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        const int quarter = warp & 3, half = warp >> 2;  // lanes of tensor memory, columns
+        const int row = quarter * 32 + lane;
+        const uint32_t taddr = tmem + (uint32_t(quarter * 32) << 16) + half * C::kCols;
+        uint32_t it = 0;
+        bool ok = true;
+        BlockWalk<BN, kGrouped> walk(p, tables, first, step);
+        BlockTile t;
+        while (ok && walk.next(t)) {
+            uint64_t acc[C::kCols / 2];
+#pragma unroll
+            for (int i = 0; i < C::kCols / 2; ++i) acc[i] = 0;
+            const bool row_ok = row < t.valid;
+            const bool busy = quarter * 32 < t.valid;  // warp-uniform
+            const float* const pa = p.sfa + int64_t(t.row0 + (row_ok ? row : 0)) * p.k_tiles;
+            const int n_block = min((t.n0 + (BN == 256 ? half * C::kCols : 0)) / 128, p.n_blocks - 1);
+            const float* const pb = kRowScales ? nullptr : p.sfb + (int64_t(t.expert) * p.n_blocks + n_block) * p.k_tiles;
+            // the scales of four k-tiles are loaded while the four before them are worked on
+            float na[4], nb[4];
+            const auto load_scales = [&](int k0) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    na[i] = nb[i] = 0.0f;
+                    if (k0 + i < k_end) {
+                        na[i] = __ldg(pa + k0 + i);
+                        if (!kRowScales) nb[i] = __ldg(pb + k0 + i);
+                    }
+                }
+            };
+            load_scales(k_begin);
+            for (int k0 = k_begin; ok && k0 < k_end; k0 += 4) {
+                float sc[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sc[i] = kRowScales ? na[i] : na[i] * nb[i];
+                load_scales(k0 + 4);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (k0 + i >= k_end) break;
+                    const uint32_t buf = it % C::kBufs, slot = it % kScaleSlots;
+                    if constexpr (kRowScales) {
+                        ok = wait_bars<true>(ptx::smem_u32(&bars->acc_full[buf]), (it / C::kBufs) & 1u, true, ptx::smem_u32(&bars->sf_full[slot]),
+                                       (it / kScaleSlots) & 1u, abort, kStatusEpilogue);
+                    } else {
+                        ok = wait_bar<true>(ptx::smem_u32(&bars->acc_full[buf]), (it / C::kBufs) & 1u, abort, kStatusEpilogue);
+                    }
+                    if (!ok) break;
+                    if (busy) {
+                        ptx::tc_fence_after();
+                        const uint64_t s2 = pack2(__float_as_uint(sc[i]), __float_as_uint(sc[i]));
+                        const float* const col_scales = scales + slot * BN + half * C::kCols;
+                        uint32_t r[2][16];
+                        load_32x16(taddr + buf * BN, r[0]);
+#pragma unroll
+                        for (int c = 0; c < C::kCols / 16; ++c) {
+                            load_wait(r[c & 1]);
+                            if (c + 1 < C::kCols / 16) load_32x16(taddr + buf * BN + (c + 1) * 16, r[(c + 1) & 1]);
+                            if (c + 1 == C::kCols / 16) {
+                                ptx::tc_fence_before();
+                                __syncwarp();
+                                if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&bars->acc_empty[buf]));
+                            }
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                uint64_t v = pack2(r[c & 1][2 * j], r[c & 1][2 * j + 1]);
+                                if constexpr (kRowScales) {
+                                    v = mul2(v, *reinterpret_cast<const uint64_t*>(col_scales + c * 16 + 2 * j));
+                                }
+                                acc[c * 8 + j] = fma2(v, s2, acc[c * 8 + j]);
+                            }
+                        }
+                    } else if (lane == 0) {
+                        ptx::mbar_arrive(ptx::smem_u32(&bars->acc_empty[buf]));
+                    }
+                    if constexpr (kRowScales) {
+                        __syncwarp();
+                        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&bars->sf_empty[slot]));
+                    }
+                    ++it;
+                }
+            }
+            if (!ok) break;
+            if constexpr (kSplit) {
+                // this CTA's sums into its own ring, which nothing uses any more (the last MMAs are done); lines of BN + 4 values
+                // keep the lanes' 16-byte stores apart
+                if (busy) {
+                    float* const line = reinterpret_cast<float*>(smem) + row * (BN + 4) + half * C::kCols;
+#pragma unroll
+                    for (int c = 0; c < C::kCols / 4; ++c) {
+                        float4 v;
+                        unpack2(acc[2 * c], v.x, v.y);
+                        unpack2(acc[2 * c + 1], v.z, v.w);
+                        *reinterpret_cast<float4*>(line + c * 4) = v;
+                    }
+                }
+            } else if (row_ok) {
+                const int col = t.n0 + half * C::kCols;
+                const int64_t at = int64_t(t.row0 + row) * p.ldo + col;
+#pragma unroll
+                for (int c = 0; c < C::kCols / 16; ++c) {
+                    if (col + c * 16 >= p.n) break;
+                    float f[16];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) unpack2(acc[c * 8 + j], f[2 * j], f[2 * j + 1]);
+                    store_values<16>(f, p.out, at + c * 16, p.n - col - c * 16, p.out_type, p.out_align);
+                }
+            }
+        }
+    }
+
+    if constexpr (kSplit) {
+        // One tile per cluster: every CTA adds up its share of the tile over the CTAs, in their order.
+        __syncwarp();
+        ptx::cluster_sync();
+        if (warp < kPromoWarps) {
+            BlockWalk<BN, kGrouped> walk(p, tables, first, step);
+            BlockTile t;
+            if (walk.next(t)) {
+                constexpr int kVecs = BN / 4;
+                const int total = t.valid * kVecs;
+                const int end = int(int64_t(total) * (rank + 1) / p.split);
+                for (int i = int(int64_t(total) * rank / p.split) + threadIdx.x; i < end; i += kPromoWarps * 32) {
+                    const int r = i / kVecs, c = (i - r * kVecs) * 4;
+                    const uint32_t addr = a_base + (r * (BN + 4) + c) * 4;
+                    float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int s = 0; s < p.split; ++s) {
+                        float v[4];
+                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
+                                     : "r"(ptx::mapa_cluster(addr, s))
+                                     : "memory");
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) f[j] += v[j];
+                    }
+                    if (t.n0 + c < p.n) {
+                        store_values<4>(f, p.out, int64_t(t.row0 + r) * p.ldo + t.n0 + c, p.n - t.n0 - c, p.out_type, p.out_align);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    }
+    if (*abort != 0u) {
+        // bounded grace period for copies and MMAs in flight before the memory they target is released
+        for (int i = 0; i < 64; ++i) __nanosleep(1000);
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    // no CTA leaves while another reads its sums
+    if constexpr (kSplit) ptx::cluster_sync();
+    if (warp == 9) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc<1>(tmem, C::kTmemCols);
+    }
+}
+
+// ---------------------------------------------------------------------------- host
+
+struct BlockProblem {
+    const void* a;
+    const void* b;
+    int64_t rows_a, n, k, experts;
+    bool row_scales, grouped;
+    BlockArgs args;
+    int sms;
+    cudaStream_t stream;
+};
+
+template <int BN, bool kRowScales, bool kGrouped, bool kSplit>
+int launch_block_gemm(const BlockProblem& g, char* err, size_t errlen) {
+    using C = BlockCfg<BN, kRowScales>;
+    static SmemOptIn opt_in;
+    const auto kernel = block_gemm_kernel<BN, kRowScales, kGrouped, kSplit>;
+    HQ_CUDA_TRY(opt_in.ensure(kernel, C::kSmemBytes));
+    BlockArgs p = g.args;
+    p.tiles_m = int((g.rows_a + kTileM - 1) / kTileM);
+    p.tiles_n = int((g.n + BN - 1) / BN);
+    CUtensorMap tm_a, tm_b;
+    if (!make_tmap_2d(&tm_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.a, uint64_t(g.k), uint64_t(g.rows_a), uint64_t(g.k), kBlockK,
+                      uint32_t(p.box_rows), CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !make_tmap_2d(&tm_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.b, uint64_t(g.k), uint64_t(g.n * g.experts), uint64_t(g.k), kBlockK, BN,
+                      CU_TENSOR_MAP_SWIZZLE_128B)) {
+        return fail(err, errlen, HQ_ERR_CUDA, "cuTensorMapEncodeTiled failed for the GEMM operands");
+    }
+    // grouped: a run may add a tile to those that its rows fill
+    const int64_t row_tiles = kGrouped ? std::min<int64_t>(g.rows_a, g.rows_a / kTileM + g.experts) : p.tiles_m;
+    const int64_t tiles = row_tiles * p.tiles_n;
+    if (!kSplit) p.split = 1;
+    const int64_t grid = kSplit ? tiles * p.split : std::min<int64_t>(tiles, g.sms);
+    HQ_CUDA_TRY(launch(kernel, dim3(unsigned(grid)), dim3(C::kThreads), size_t(C::kSmemBytes), g.stream, p.pdl != 0,
+                       kSplit ? unsigned(p.split) : 1u, tm_a, tm_b, p));
+    return HQ_OK;
+}
+
+// The tile, and the CTAs that share one.
+struct BlockChoice {
+    int bn, split;
+};
+
+BlockChoice choose(const BlockProblem& g) {
+    const int k_tiles = g.args.k_tiles;
+    // microseconds of a k-tile and of a tile's end
+    struct Cost {
+        int bn;
+        double step, tile;
+    };
+    constexpr Cost kCosts[] = {{256, 0.36, 2.0}, {128, 0.22, 1.5}, {64, 0.15, 1.2}};
+    BlockChoice best = {64, 1};
+    double least = 1e30;
+    for (const Cost& c : kCosts) {
+        if (g.row_scales && c.bn == 256) continue;
+        int64_t row_tiles = (g.rows_a + kTileM - 1) / kTileM;
+        if (g.grouped) row_tiles = g.rows_a / kTileM + std::min<int64_t>(g.experts, g.rows_a);
+        const int64_t tiles = row_tiles * ((g.n + c.bn - 1) / c.bn);
+        int split = 1;
+        if (!g.grouped && !g.row_scales && c.bn <= 128) {
+            while (split < 8 && 2 * split * tiles <= g.sms && k_tiles >= 4 * split) split *= 2;
+        }
+        const double waves = double((tiles * split + g.sms - 1) / g.sms);
+        const double t = waves * (c.step * ((k_tiles + split - 1) / split) + c.tile) + (split > 1 ? 2.0 : 0.0);
+        if (t < least) least = t, best = {c.bn, split};
+    }
+    return best;
+}
+
+template <int BN, bool kRowScales>
+int launch_kind(const BlockProblem& g, char* err, size_t errlen) {
+    if constexpr (kRowScales) {
+        return launch_block_gemm<BN, true, false, false>(g, err, errlen);
+    } else {
+        if (g.grouped) return launch_block_gemm<BN, false, true, false>(g, err, errlen);
+        if constexpr (BN <= 128) {
+            if (g.args.split > 1) return launch_block_gemm<BN, false, false, true>(g, err, errlen);
+        }
+        return launch_block_gemm<BN, false, false, false>(g, err, errlen);
+    }
+}
+
+int block_gemm(const void* a, const void* b, const float* sfa, const float* sfb, const int32_t* offsets, void* out, int out_type, int64_t m,
+               int64_t n, int64_t k, int64_t experts, int row_scales, bool grouped, int64_t ldo, int sm_count, int use_pdl, int device,
+               void* stream, char* err, size_t errlen) {
+    if (out_type != HQ_DTYPE_BF16 && out_type != HQ_DTYPE_FP16 && out_type != HQ_DTYPE_FP32) {
+        return fail(err, errlen, HQ_ERR_INVALID, "output dtype must be bfloat16, float16 or float32");
+    }
+    if (m < 0 || n < 0 || experts < 0 || m > INT32_MAX - 128 || n > INT32_MAX - 256) {
+        return fail(err, errlen, HQ_ERR_INVALID, "at most 2^31 - 256 rows and columns, got M=%lld, N=%lld", static_cast<long long>(m),
+                    static_cast<long long>(n));
+    }
+    if (k < 16 || k % 16 != 0 || k > (int64_t(1) << 30)) {
+        return fail(err, errlen, HQ_ERR_INVALID, "K must be a positive multiple of 16, got K=%lld", static_cast<long long>(k));
+    }
+    if (experts > kMaxExperts || experts * n > INT32_MAX - 256) {
+        return fail(err, errlen, HQ_ERR_INVALID, "at most %d experts and 2^31 - 256 weight rows, got %lld of %lld", kMaxExperts,
+                    static_cast<long long>(experts), static_cast<long long>(n));
+    }
+    if (((m + 127) / 128 + experts) * ((n + 63) / 64) > INT32_MAX / 8) {
+        return fail(err, errlen, HQ_ERR_INVALID, "the output has too many tiles, got M=%lld, N=%lld", static_cast<long long>(m),
+                    static_cast<long long>(n));
+    }
+    if (m == 0 || n == 0 || experts == 0) return HQ_OK;
+    if (a == nullptr || b == nullptr || sfa == nullptr || sfb == nullptr || out == nullptr || (grouped && offsets == nullptr)) {
+        return fail(err, errlen, HQ_ERR_INVALID, "null pointer argument");
+    }
+    if (!aligned(a, 16) || !aligned(b, 16)) return fail(err, errlen, HQ_ERR_INVALID, "input and weight must be 16-byte aligned");
+    const int size = out_type == HQ_DTYPE_FP32 ? 4 : 2;
+    if (ldo < n || !aligned(sfa, 4) || !aligned(sfb, 4) || !aligned(out, size_t(size))) {
+        return fail(err, errlen, HQ_ERR_INVALID, "output rows must hold N values, got a row stride of %lld", static_cast<long long>(ldo));
+    }
+    const DeviceGuard guard(device);
+    if (!guard.ok()) return fail(err, errlen, HQ_ERR_CUDA, "cannot select CUDA device %d", device);
+    const int sms = hq_sm_count(device);
+    if (sms <= 0) return fail(err, errlen, HQ_ERR_CUDA, "cannot read the SM count of CUDA device %d", device);
+    BlockProblem g = {};
+    g.a = a, g.b = b, g.rows_a = m, g.n = n, g.k = k, g.experts = experts, g.row_scales = row_scales != 0, g.grouped = grouped;
+    g.sms = sm_count > 0 ? std::min(sm_count, sms) : sms;
+    g.stream = static_cast<cudaStream_t>(stream);
+    BlockArgs& p = g.args;
+    p.sfa = sfa, p.sfb = sfb, p.out = out, p.offsets = offsets, p.ldo = ldo;
+    p.m = int(m), p.n = int(n), p.k_tiles = int((k + kBlockK - 1) / kBlockK);
+    p.n_blocks = int((n + 127) / 128), p.experts = int(experts), p.out_type = out_type, p.pdl = use_pdl != 0;
+    const int64_t row_bytes = ldo * size;
+    p.out_align = aligned(out, 32) && row_bytes % 32 == 0 ? 32 : aligned(out, 16) && row_bytes % 16 == 0 ? 16 : size;
+    // Rows of `a` per copy: all of a tile's, or about those of a run, so that short runs do not read their neighbours' rows.
+    const int64_t mean = grouped ? (m + std::min(experts, m) - 1) / std::min(experts, m) : m;
+    p.box_rows = 8;
+    while (p.box_rows < kTileM && p.box_rows < mean) p.box_rows *= 2;
+    const BlockChoice c = choose(g);
+    p.split = c.split;
+    if (g.row_scales) return c.bn == 128 ? launch_kind<128, true>(g, err, errlen) : launch_kind<64, true>(g, err, errlen);
+    return c.bn == 256   ? launch_kind<256, false>(g, err, errlen)
+           : c.bn == 128 ? launch_kind<128, false>(g, err, errlen)
+                         : launch_kind<64, false>(g, err, errlen);
+}
+
+}  // namespace
+
+// Reads and clears this file's status word; the stream has been synchronised.
+cudaError_t take_block_gemm_status(uint32_t* status) {
+    uint32_t host[4] = {0, 0, 0, 0};
+    cudaError_t e = cudaMemcpyFromSymbol(host, g_status, sizeof(host));
+    if (e == cudaSuccess && host[0] != 0) {
+        const uint32_t zero[4] = {0, 0, 0, 0};
+        e = cudaMemcpyToSymbol(g_status, zero, sizeof(zero));
+    }
+    *status = host[0];
+    return e;
+}
+
+}  // namespace hq
+
+extern "C" int hq_block_gemm(const void* a, const void* b, const float* sfa, const float* sfb, void* out, int out_dtype, int64_t m, int64_t n,
+                             int64_t k, int row_scales, int64_t ldo, int sm_count, int use_pdl, int device, void* stream, char* err,
+                             size_t errlen) {
+    return hq::block_gemm(a, b, sfa, sfb, nullptr, out, out_dtype, m, n, k, 1, row_scales, false, ldo, sm_count, use_pdl, device, stream, err,
+                          errlen);
+}
+
+extern "C" int hq_group_block_gemm(const void* a, const void* b, const float* sfa, const float* sfb, const int32_t* offsets, void* out,
+                                   int out_dtype, int64_t num_experts, int64_t m, int64_t n, int64_t k, int64_t ldo, int sm_count, int use_pdl,
+                                   int device, void* stream, char* err, size_t errlen) {
+    return hq::block_gemm(a, b, sfa, sfb, offsets, out, out_dtype, m, n, k, num_experts, 0, true, ldo, sm_count, use_pdl, device, stream, err,
+                          errlen);
+}

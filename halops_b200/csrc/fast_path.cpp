@@ -20,7 +20,9 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cstring>
+#include <type_traits>
 
 #include "../../include/halops_b200.h"
 
@@ -47,6 +49,15 @@ struct {
     MaskedFn masked;
     ContiguousFn contiguous;
     decltype(&hq_hold_switches) hold_switches;
+    decltype(&hq_block_quant) block_quant;
+    decltype(&hq_swiglu_block_quant) swiglu;
+    decltype(&hq_block_gemm) block_gemm;
+    decltype(&hq_group_block_gemm) group_block_gemm;
+    decltype(&hq_moe_sort) moe_sort;
+    decltype(&hq_moe_permute) moe_permute;
+    decltype(&hq_moe_permute_block_quant) moe_permute_quant;
+    decltype(&hq_moe_unpermute) moe_unpermute;
+    decltype(&hq_moe_unpermute_backward) moe_unpermute_backward;
 } g_fn;
 
 // the package's mode names
@@ -233,6 +244,388 @@ PyObject* rms_norm_quant(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- FP8 with a scale per block of 128, tokens in expert order
+
+int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
+
+int in_dtype(const at::Tensor& t) {
+    return t.scalar_type() == at::kBFloat16 ? HQ_DTYPE_BF16 : t.scalar_type() == at::kHalf ? HQ_DTYPE_FP16 : -1;
+}
+int any_dtype(const at::Tensor& t) { return t.scalar_type() == at::kFloat ? HQ_DTYPE_FP32 : in_dtype(t); }
+
+// rows of 16-bit elements as the kernels read them
+bool rows16(const at::Tensor& x) {
+    if (x.stride(-1) != 1 || reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 != 0) return false;
+    for (int64_t i = 0; i + 1 < x.dim(); ++i) {
+        if (x.stride(i) % 8 != 0) return false;
+    }
+    return true;
+}
+
+// An output that the caller may have given: false if it is not what it should be.
+bool given(PyObject* o, c10::IntArrayRef shape, at::ScalarType type, const at::Tensor& like, at::Tensor* out) {
+    if (o == Py_None) return true;
+    const at::Tensor* const t = plain_tensor(o);
+    if (t == nullptr || !t->is_contiguous() || t->scalar_type() != type || t->sizes() != shape || t->device() != like.device()) return false;
+    *out = *t;
+    return true;
+}
+
+PyObject* pair_or_given(PyObject* a, const at::Tensor& x, PyObject* b, const at::Tensor& y) {
+    PyObject* const p = a != Py_None ? Py_NewRef(a) : THPVariable_Wrap(x);
+    PyObject* const q = p == nullptr ? nullptr : b != Py_None ? Py_NewRef(b) : THPVariable_Wrap(y);
+    PyObject* const t = q != nullptr ? PyTuple_Pack(2, p, q) : nullptr;
+    Py_XDECREF(p);
+    Py_XDECREF(q);
+    return t;
+}
+
+// block_quant(input, block, transpose, use_pdl, output_quant, output_sf)
+PyObject* block_quant(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    int transpose, pdl, rows, cols;
+    if (nargs != 6 || g_fn.block_quant == nullptr || at::impl::torch_function_mode_enabled()) Py_RETURN_NONE;
+    const at::Tensor* const x = plain_tensor(a[0]);
+    if (x == nullptr || !PyTuple_CheckExact(a[1]) || PyTuple_GET_SIZE(a[1]) != 2 || !small_int(PyTuple_GET_ITEM(a[1], 0), &rows) ||
+        !small_int(PyTuple_GET_ITEM(a[1], 1), &cols) || !flag(a[2], &transpose) || !flag(a[3], &pdl)) {
+        Py_RETURN_NONE;
+    }
+    if (cols != 128 || (rows != 1 && rows != 128) || !(x->dim() == 2 || (rows == 128 && x->dim() == 3))) Py_RETURN_NONE;
+    const int type = in_dtype(*x);
+    const int64_t m = x->size(-2), k = x->size(-1), e = x->dim() == 3 ? x->size(0) : 1;
+    if (type < 0 || k % 16 != 0 || !rows16(*x)) Py_RETURN_NONE;
+    const int64_t m16 = (m + 15) / 16 * 16, r = transpose ? k : m, c = transpose ? m : k;
+    const int64_t q_shape[3] = {e, r, transpose ? m16 : k}, s_shape[3] = {e, rows == 128 ? blocks_of(r) : r, blocks_of(c)};
+    const size_t skip = x->dim() == 3 ? 0 : 1;
+    const c10::IntArrayRef qs(q_shape + skip, 3 - skip), ss(s_shape + skip, 3 - skip);
+    at::Tensor q, sf;
+    if (!given(a[4], qs, at::kFloat8_e4m3fn, *x, &q) || !given(a[5], ss, at::kFloat, *x, &sf)) Py_RETURN_NONE;
+    const void* const px = x->data_ptr();
+    const int64_t ld = x->stride(-2), batch = x->dim() == 3 ? x->stride(0) : 0;
+    const int dev = x->get_device();
+    void* const st = stream_of(*x);
+    const auto on_device = at::TensorOptions().device(x->device());
+    if (unlocked([&](char* err) {
+            if (!q.defined()) q = at::empty(qs, on_device.dtype(at::kFloat8_e4m3fn));
+            if (!sf.defined()) sf = at::empty(ss, on_device.dtype(at::kFloat));
+            return g_fn.block_quant(px, ld, batch, type, e, m, k, rows, transpose, pdl, q.data_ptr(), sf.data_ptr(), dev, st, err, kErrLen);
+        }) != 0) {
+        Py_RETURN_NONE;
+    }
+    return pair_or_given(a[4], q, a[5], sf);
+    END_HANDLE_TH_ERRORS
+}
+
+// swiglu_block_quant(input, offsets, use_pdl, output_quant, output_sf)
+PyObject* swiglu_block_quant(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    int pdl;
+    if (nargs != 5 || g_fn.swiglu == nullptr || at::impl::torch_function_mode_enabled()) Py_RETURN_NONE;
+    const at::Tensor* const x = plain_tensor(a[0]);
+    if (x == nullptr || x->dim() != 2 || !flag(a[2], &pdl)) Py_RETURN_NONE;
+    const int type = in_dtype(*x);
+    const int64_t m = x->size(0), k = x->size(1) / 2;
+    if (type < 0 || x->size(1) % 32 != 0 || !rows16(*x)) Py_RETURN_NONE;
+    const int32_t* limit = nullptr;
+    if (a[1] != Py_None) {
+        const at::Tensor* const o = plain_tensor(a[1]);
+        if (o == nullptr || o->dim() != 1 || o->size(0) < 1 || o->scalar_type() != at::kInt || !o->is_contiguous() || o->device() != x->device()) {
+            Py_RETURN_NONE;
+        }
+        limit = static_cast<const int32_t*>(o->data_ptr()) + (o->size(0) - 1);
+    }
+    const int64_t qs[2] = {m, k}, ss[2] = {m, blocks_of(k)};
+    at::Tensor q, sf;
+    if (!given(a[3], qs, at::kFloat8_e4m3fn, *x, &q) || !given(a[4], ss, at::kFloat, *x, &sf)) Py_RETURN_NONE;
+    const void* const px = x->data_ptr();
+    const int64_t ld = x->stride(0);
+    const int dev = x->get_device();
+    void* const st = stream_of(*x);
+    const auto on_device = at::TensorOptions().device(x->device());
+    if (unlocked([&](char* err) {
+            if (!q.defined()) q = at::empty(qs, on_device.dtype(at::kFloat8_e4m3fn));
+            if (!sf.defined()) sf = at::empty(ss, on_device.dtype(at::kFloat));
+            return g_fn.swiglu(px, ld, type, m, k, limit, pdl, q.data_ptr(), sf.data_ptr(), dev, st, err, kErrLen);
+        }) != 0) {
+        Py_RETURN_NONE;
+    }
+    return pair_or_given(a[3], q, a[4], sf);
+    END_HANDLE_TH_ERRORS
+}
+
+// block_gemm(input, weight, sfa, sfb, offsets or None, output, sm_count, use_pdl) -> True
+PyObject* block_gemm(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    int pdl, sm_count;
+    if (nargs != 8 || g_fn.block_gemm == nullptr || at::impl::torch_function_mode_enabled()) Py_RETURN_NONE;
+    const at::Tensor* const x = plain_tensor(a[0]);
+    const at::Tensor* const w = plain_tensor(a[1]);
+    const at::Tensor* const sfa = plain_tensor(a[2]);
+    const at::Tensor* const sfb = plain_tensor(a[3]);
+    const bool grouped = a[4] != Py_None;
+    const at::Tensor* const offsets = grouped ? plain_tensor(a[4]) : nullptr;
+    const at::Tensor* const out = plain_tensor(a[5]);
+    if (x == nullptr || w == nullptr || sfa == nullptr || sfb == nullptr || out == nullptr || (grouped && offsets == nullptr) ||
+        !small_int(a[6], &sm_count) || !flag(a[7], &pdl)) {
+        Py_RETURN_NONE;
+    }
+    if (x->dim() != 2 || w->dim() != (grouped ? 3 : 2) || sfa->dim() != 2 || sfb->dim() != w->dim() || out->dim() != 2) Py_RETURN_NONE;
+    const int64_t m = x->size(0), k = x->size(1), n = w->size(-2), e = grouped ? w->size(0) : 1, kb = blocks_of(k);
+    const int type = any_dtype(*out);
+    if (m == 0 || n == 0 || e == 0 || k < 16 || k % 16 != 0 || w->size(-1) != k || type < 0) Py_RETURN_NONE;
+    if (x->scalar_type() != at::kFloat8_e4m3fn || w->scalar_type() != at::kFloat8_e4m3fn || sfa->scalar_type() != at::kFloat ||
+        sfb->scalar_type() != at::kFloat) {
+        Py_RETURN_NONE;
+    }
+    const auto dev = x->device();
+    if (w->device() != dev || sfa->device() != dev || sfb->device() != dev || out->device() != dev) Py_RETURN_NONE;
+    if (!x->is_contiguous() || !w->is_contiguous() || !sfa->is_contiguous() || !sfb->is_contiguous()) Py_RETURN_NONE;
+    if (sfa->size(0) != m || sfa->size(1) != kb || sfb->size(-1) != kb) Py_RETURN_NONE;
+    const bool square = sfb->size(-2) == blocks_of(n);
+    if (grouped ? (!square || sfb->size(0) != e) : (!square && sfb->size(0) != n)) Py_RETURN_NONE;
+    if (out->size(0) != m || out->size(1) != n || (out->stride(1) != 1 && n > 1) || (out->stride(0) < n && m > 1)) Py_RETURN_NONE;
+    if (grouped && (offsets->dim() != 1 || offsets->scalar_type() != at::kInt || offsets->size(0) != e + 1 || !offsets->is_contiguous() ||
+                    offsets->device() != dev)) {
+        Py_RETURN_NONE;
+    }
+    const void *const px = x->data_ptr(), *const pw = w->data_ptr();
+    if (reinterpret_cast<uintptr_t>(px) % 16 != 0 || reinterpret_cast<uintptr_t>(pw) % 16 != 0) Py_RETURN_NONE;
+    const float *const pa = static_cast<const float*>(sfa->data_ptr()), *const pb = static_cast<const float*>(sfb->data_ptr());
+    const int32_t* const po = grouped ? static_cast<const int32_t*>(offsets->data_ptr()) : nullptr;
+    void* const y = out->data_ptr();
+    const int64_t ldo = std::max(out->stride(0), n);
+    const int d = x->get_device();
+    void* const st = stream_of(*x);
+    const int rc = unlocked([&](char* err) {
+        return grouped ? g_fn.group_block_gemm(px, pw, pa, pb, po, y, type, e, m, n, k, ldo, sm_count, pdl, d, st, err, kErrLen)
+                       : g_fn.block_gemm(px, pw, pa, pb, y, type, m, n, k, square ? 0 : 1, ldo, sm_count, pdl, d, st, err, kErrLen);
+    });
+    if (rc != 0) Py_RETURN_NONE;
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// moe_sort(topk_ids, num_experts, align, use_pdl) -> (rows, pairs, offsets, expert_ids)
+PyObject* moe_sort(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    int experts, align, pdl;
+    if (nargs != 4 || g_fn.moe_sort == nullptr || at::impl::torch_function_mode_enabled()) Py_RETURN_NONE;
+    const at::Tensor* const ids = plain_tensor(a[0]);
+    if (ids == nullptr || ids->dim() != 2 || !ids->is_contiguous() || !small_int(a[1], &experts) || !small_int(a[2], &align) || !flag(a[3], &pdl)) {
+        Py_RETURN_NONE;
+    }
+    if ((ids->scalar_type() != at::kInt && ids->scalar_type() != at::kLong) || experts < 1 || experts > 1024 || align < 1 || align > 65536) {
+        Py_RETURN_NONE;
+    }
+    const int64_t n = ids->numel(), n_rows = (n + std::min<int64_t>(experts, n) * (align - 1)) / align * align;
+    if (n_rows > INT32_MAX) Py_RETURN_NONE;
+    const void* const p = ids->data_ptr();
+    const int dev = ids->get_device();
+    void* const st = stream_of(*ids);
+    const auto options = at::TensorOptions().device(ids->device()).dtype(at::kInt);
+    at::Tensor out[4];
+    if (unlocked([&](char* err) {
+            out[0] = at::empty(ids->sizes(), options);
+            out[1] = at::empty({n_rows}, options);
+            out[2] = at::empty({experts + 1}, options);
+            out[3] = at::empty({n_rows}, options);
+            int32_t* at[4];
+            for (int i = 0; i < 4; ++i) at[i] = static_cast<int32_t*>(out[i].data_ptr());
+            return g_fn.moe_sort(p, int(ids->element_size()), ids->size(0), ids->size(1), experts, align, n_rows, pdl, at[0], at[1], at[2], at[3],
+                                 dev, st, err, kErrLen);
+        }) != 0) {
+        Py_RETURN_NONE;
+    }
+    PyObject* const t = PyTuple_New(4);
+    for (int i = 0; t != nullptr && i < 4; ++i) {
+        PyObject* const v = THPVariable_Wrap(out[i]);
+        if (v == nullptr) {
+            Py_DECREF(t);
+            return nullptr;
+        }
+        PyTuple_SET_ITEM(t, i, v);
+    }
+    return t;
+    END_HANDLE_TH_ERRORS
+}
+
+// the fields of a MoeSort
+struct Order {
+    const int32_t *rows, *pairs, *offsets;
+    int64_t tokens, topk, n_rows, experts;
+    int padded;
+
+    bool read(PyObject* o, c10::Device device) {
+        if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 5) return false;
+        const at::Tensor* t[3];
+        for (int i = 0; i < 3; ++i) {
+            t[i] = plain_tensor(PyTuple_GET_ITEM(o, i));
+            if (t[i] == nullptr || t[i]->dim() != (i == 0 ? 2 : 1) || t[i]->scalar_type() != at::kInt || !t[i]->is_contiguous() ||
+                t[i]->device() != device) {
+                return false;
+            }
+        }
+        int align;
+        if (!small_int(PyTuple_GET_ITEM(o, 4), &align) || t[2]->size(0) < 1) return false;
+        rows = static_cast<const int32_t*>(t[0]->data_ptr());
+        pairs = static_cast<const int32_t*>(t[1]->data_ptr());
+        offsets = static_cast<const int32_t*>(t[2]->data_ptr());
+        tokens = t[0]->size(0), topk = t[0]->size(1), n_rows = t[1]->size(0), experts = t[2]->size(0) - 1;
+        padded = align > 1 ? 1 : 0;
+        return true;
+    }
+};
+
+// moe_permute(input, sort, output, use_pdl)
+PyObject* moe_permute(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    int pdl;
+    Order order;
+    if (nargs != 4 || g_fn.moe_permute == nullptr || at::impl::torch_function_mode_enabled()) Py_RETURN_NONE;
+    const at::Tensor* const x = plain_tensor(a[0]);
+    if (x == nullptr || x->dim() != 2 || (x->stride(1) != 1 && x->size(1) > 1) || !order.read(a[1], x->device()) || !flag(a[3], &pdl)) Py_RETURN_NONE;
+    const int64_t size = x->element_size(), h = x->size(1);
+    if ((size != 1 && size != 2 && size != 4) || x->size(0) != order.tokens) Py_RETURN_NONE;
+    const int64_t shape[2] = {order.n_rows, h};
+    at::Tensor out;
+    if (!given(a[2], shape, x->scalar_type(), *x, &out)) Py_RETURN_NONE;
+    const void* const px = x->data_ptr();
+    const int64_t ld = x->stride(0) * size;
+    const int dev = x->get_device();
+    void* const st = stream_of(*x);
+    if (unlocked([&](char* err) {
+            if (!out.defined()) out = at::empty(shape, x->options());
+            return g_fn.moe_permute(px, ld, order.tokens, h * size, order.topk, order.rows, order.pairs, order.offsets, order.experts, order.n_rows,
+                                    order.padded, pdl, out.data_ptr(), dev, st, err, kErrLen);
+        }) != 0) {
+        Py_RETURN_NONE;
+    }
+    return a[2] != Py_None ? Py_NewRef(a[2]) : THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// moe_permute_block_quant(input, sort, use_pdl, output_quant, output_sf)
+PyObject* moe_permute_block_quant(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    int pdl;
+    Order order;
+    if (nargs != 5 || g_fn.moe_permute_quant == nullptr || at::impl::torch_function_mode_enabled()) Py_RETURN_NONE;
+    const at::Tensor* const x = plain_tensor(a[0]);
+    if (x == nullptr || x->dim() != 2 || !order.read(a[1], x->device()) || !flag(a[2], &pdl)) Py_RETURN_NONE;
+    const int type = in_dtype(*x);
+    const int64_t h = x->size(1);
+    if (type < 0 || h % 16 != 0 || !rows16(*x) || x->size(0) != order.tokens) Py_RETURN_NONE;
+    const int64_t qs[2] = {order.n_rows, h}, ss[2] = {order.n_rows, blocks_of(h)};
+    at::Tensor q, sf;
+    if (!given(a[3], qs, at::kFloat8_e4m3fn, *x, &q) || !given(a[4], ss, at::kFloat, *x, &sf)) Py_RETURN_NONE;
+    const void* const px = x->data_ptr();
+    const int64_t ld = x->stride(0);
+    const int dev = x->get_device();
+    void* const st = stream_of(*x);
+    const auto on_device = at::TensorOptions().device(x->device());
+    if (unlocked([&](char* err) {
+            if (!q.defined()) q = at::empty(qs, on_device.dtype(at::kFloat8_e4m3fn));
+            if (!sf.defined()) sf = at::empty(ss, on_device.dtype(at::kFloat));
+            return g_fn.moe_permute_quant(px, ld, type, order.tokens, h, order.topk, order.rows, order.pairs, order.offsets, order.experts,
+                                          order.n_rows, order.padded, pdl, q.data_ptr(), sf.data_ptr(), dev, st, err, kErrLen);
+        }) != 0) {
+        Py_RETURN_NONE;
+    }
+    return pair_or_given(a[3], q, a[4], sf);
+    END_HANDLE_TH_ERRORS
+}
+
+// the weights of the pairs, or none
+bool pair_weights(PyObject* o, const Order& order, c10::Device device, const float** weights) {
+    *weights = nullptr;
+    if (o == Py_None) return true;
+    const at::Tensor* const t = plain_tensor(o);
+    if (t == nullptr || t->scalar_type() != at::kFloat || t->dim() != 2 || t->size(0) != order.tokens || t->size(1) != order.topk ||
+        !t->is_contiguous() || t->device() != device) {
+        return false;
+    }
+    *weights = static_cast<const float*>(t->data_ptr());
+    return true;
+}
+
+// moe_unpermute(input, sort, weights, use_pdl)
+PyObject* moe_unpermute(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    int pdl;
+    Order order;
+    const float* weights;
+    if (nargs != 4 || g_fn.moe_unpermute == nullptr || at::impl::torch_function_mode_enabled()) Py_RETURN_NONE;
+    const at::Tensor* const z = plain_tensor(a[0]);
+    if (z == nullptr || z->dim() != 2 || (z->stride(1) != 1 && z->size(1) > 1) || !order.read(a[1], z->device()) ||
+        !pair_weights(a[2], order, z->device(), &weights) || !flag(a[3], &pdl)) {
+        Py_RETURN_NONE;
+    }
+    const int type = any_dtype(*z);
+    const int64_t h = z->size(1);
+    if (type < 0 || z->size(0) != order.n_rows) Py_RETURN_NONE;
+    const void* const pz = z->data_ptr();
+    const int64_t ld = z->stride(0);
+    const int dev = z->get_device();
+    void* const st = stream_of(*z);
+    at::Tensor out;
+    if (unlocked([&](char* err) {
+            out = at::empty({order.tokens, h}, z->options());
+            return g_fn.moe_unpermute(pz, ld, type, order.n_rows, h, order.tokens, order.topk, order.rows, weights, pdl, out.data_ptr(), dev, st, err,
+                                      kErrLen);
+        }) != 0) {
+        Py_RETURN_NONE;
+    }
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// moe_unpermute_backward(grad_output, input, sort, weights, use_pdl, grad_input)
+PyObject* moe_unpermute_backward(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    int pdl;
+    Order order;
+    const float* weights;
+    if (nargs != 6 || g_fn.moe_unpermute_backward == nullptr || at::impl::torch_function_mode_enabled()) Py_RETURN_NONE;
+    const at::Tensor* const g = plain_tensor(a[0]);
+    const at::Tensor* const z = plain_tensor(a[1]);
+    if (g == nullptr || z == nullptr || g->dim() != 2 || z->dim() != 2 || (z->stride(1) != 1 && z->size(1) > 1) ||
+        (g->stride(1) != 1 && g->size(1) > 1) || !order.read(a[2], z->device()) || !pair_weights(a[3], order, z->device(), &weights) ||
+        !flag(a[4], &pdl)) {
+        Py_RETURN_NONE;
+    }
+    const int type = any_dtype(*z);
+    const int64_t h = z->size(1);
+    if (type < 0 || g->scalar_type() != z->scalar_type() || g->device() != z->device() || z->size(0) != order.n_rows || g->size(0) != order.tokens ||
+        g->size(1) != h) {
+        Py_RETURN_NONE;
+    }
+    const int64_t shape[2] = {order.n_rows, h};
+    at::Tensor gz, gw;
+    if (!given(a[5], shape, z->scalar_type(), *z, &gz)) Py_RETURN_NONE;
+    const void *const pg = g->data_ptr(), *const pz = z->data_ptr();
+    const int64_t ld_g = g->stride(0), ld_z = z->stride(0);
+    const int dev = z->get_device();
+    void* const st = stream_of(*z);
+    if (unlocked([&](char* err) {
+            if (!gz.defined()) gz = at::empty(shape, z->options());
+            if (a[3] != Py_None) gw = at::empty({order.tokens, order.topk}, z->options().dtype(at::kFloat));
+            return g_fn.moe_unpermute_backward(pg, ld_g, pz, ld_z, type, order.n_rows, h, order.tokens, order.topk, order.rows, order.pairs,
+                                               order.offsets, order.experts, order.padded, weights, pdl, gz.data_ptr(),
+                                               gw.defined() ? static_cast<float*>(gw.data_ptr()) : nullptr, dev, st, err, kErrLen);
+        }) != 0) {
+        Py_RETURN_NONE;
+    }
+    PyObject* const p = a[5] != Py_None ? Py_NewRef(a[5]) : THPVariable_Wrap(gz);
+    PyObject* const q = p == nullptr ? nullptr : gw.defined() ? THPVariable_Wrap(gw) : Py_NewRef(Py_None);
+    PyObject* const t = q != nullptr ? PyTuple_Pack(2, p, q) : nullptr;
+    Py_XDECREF(p);
+    Py_XDECREF(q);
+    return t;
+    END_HANDLE_TH_ERRORS
+}
+
+// ---- GEMMs with block scales of the MX kinds: they read environment switches
+
 // dense_gemm(input, weight, sfa, sfb, output, bias, alpha, sm_count, mode, use_pdl, epilogue, output_sf,
 //            situ_beta, situ_linear_beta) -> True, or None when the call is not an ordinary one
 PyObject* dense_gemm(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
@@ -391,6 +784,24 @@ PyObject* grouped_gemm(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// bind_block(block_quant, swiglu, block_gemm, group_block_gemm, moe_sort, moe_permute, moe_permute_quant, moe_unpermute,
+// moe_unpermute_backward): addresses, as for bind
+PyObject* bind_block(PyObject*, PyObject* args) {
+    unsigned long long p[9];
+    if (!PyArg_ParseTuple(args, "KKKKKKKKK", &p[0], &p[1], &p[2], &p[3], &p[4], &p[5], &p[6], &p[7], &p[8])) return nullptr;
+    const auto set = [&](auto& fn, int i) { fn = reinterpret_cast<std::remove_reference_t<decltype(fn)>>(p[i]); };
+    set(g_fn.block_quant, 0);
+    set(g_fn.swiglu, 1);
+    set(g_fn.block_gemm, 2);
+    set(g_fn.group_block_gemm, 3);
+    set(g_fn.moe_sort, 4);
+    set(g_fn.moe_permute, 5);
+    set(g_fn.moe_permute_quant, 6);
+    set(g_fn.moe_unpermute, 7);
+    set(g_fn.moe_unpermute_backward, 8);
+    Py_RETURN_NONE;
+}
+
 // bind(quant, rms, dense, situ, describe_group, masked, contiguous, hold_switches): addresses of the C ABI's entry points
 PyObject* bind(PyObject*, PyObject* args) {
     unsigned long long p[8];
@@ -415,7 +826,16 @@ PyMethodDef methods[] = {{"group_wise_quant", method(group_wise_quant), METH_FAS
                          {"rms_norm_quant", method(rms_norm_quant), METH_FASTCALL, nullptr},
                          {"dense_gemm", method(dense_gemm), METH_FASTCALL, nullptr},
                          {"grouped_gemm", method(grouped_gemm), METH_FASTCALL, nullptr},
+                         {"block_quant", method(block_quant), METH_FASTCALL, nullptr},
+                         {"swiglu_block_quant", method(swiglu_block_quant), METH_FASTCALL, nullptr},
+                         {"block_gemm", method(block_gemm), METH_FASTCALL, nullptr},
+                         {"moe_sort", method(moe_sort), METH_FASTCALL, nullptr},
+                         {"moe_permute", method(moe_permute), METH_FASTCALL, nullptr},
+                         {"moe_permute_block_quant", method(moe_permute_block_quant), METH_FASTCALL, nullptr},
+                         {"moe_unpermute", method(moe_unpermute), METH_FASTCALL, nullptr},
+                         {"moe_unpermute_backward", method(moe_unpermute_backward), METH_FASTCALL, nullptr},
                          {"bind", bind, METH_VARARGS, nullptr},
+                         {"bind_block", bind_block, METH_VARARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "halops_b200_fast_path", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -1,0 +1,586 @@
+// Tokens in the order of the experts that a router gave them, and back.
+//
+// A pair p = token * topk + slot has an expert ids[p]; one outside of [0, experts) is dropped (it belongs to another device).
+// The pairs of an expert keep their order and become a run of rows that starts on a multiple of `align`:
+//   offsets[e]     first row of expert e's run; offsets[experts] is the end of the last
+//   rows[p]        the pair's row, -1 for a dropped one
+//   pairs[r]       the row's pair, -1 for a row that pads a run or lies behind the last
+//   expert_ids[r]  the run that row r is in, experts - 1 behind the last run
+//
+// The sort is one launch; what moves tokens is bound by HBM: every token is read once and written once per expert,
+// or the other way round.
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include <mutex>
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace hq {
+namespace {
+
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// ---------------------------------------------------------------------------- sort
+//
+// A stable counting sort by one cluster of 1 or 8 CTAs.  Every warp has a stretch of the pairs: it counts their experts into a
+// line of its own in shared memory, the lines are summed over the warps of the CTA and, through distributed shared memory, over the
+// CTAs before this one, and then the warp goes over its stretch again, 32 pairs at a time: a pair's row is its expert's
+// start plus the pairs of that expert before it, counted in the warp's line and, among the 32, by a match of the lanes.  All
+// counts are whole numbers, so the order in which warps run changes nothing.
+
+constexpr int kSortThreads = 1024;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kMaxExperts = 1024;
+
+template <typename Id>
+__device__ __forceinline__ int expert_of(const Id* ids, int p, int pairs_n, int experts) {
+    if (p >= pairs_n) return -1;
+    const Id id = ids[p];
+    return id >= 0 && id < Id(experts) ? int(id) : -1;
+}
+
+template <typename Id>
+__global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const Id* __restrict__ ids, int pairs_n, int experts, int align, int n_rows,
+                                                                int ctas, int* __restrict__ rows, int* __restrict__ pairs,
+                                                                int* __restrict__ offsets, int* __restrict__ expert_ids) {
+    extern __shared__ int smem[];
+    int* const lines = smem;                             // [warp][expert]
+    int* const total = lines + kSortWarps * experts;     // this CTA's pairs per expert, read by the cluster
+    int* const count = total + experts;                  // all pairs per expert
+    int* const start = count + experts;                  // first row of the expert's run, and the end of the last
+    __shared__ int warp_sums[kSortWarps];
+    grid_wait();
+    grid_launch_dependents();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x;
+    for (int i = tid; i < kSortWarps * experts; i += kSortThreads) lines[i] = 0;
+    __syncthreads();
+
+    const int stretch = (pairs_n + ctas * kSortWarps - 1) / (ctas * kSortWarps);
+    const int64_t first = int64_t(cta * kSortWarps + warp) * stretch;
+    const int begin = int(min(first, int64_t(pairs_n))), end = int(min(first + stretch, int64_t(pairs_n)));
+    int* const line = lines + warp * experts;
+    for (int p = begin + lane; p < end; p += 32) {
+        const int e = expert_of(ids, p, end, experts);
+        if (e >= 0) atomicAdd(line + e, 1);
+    }
+    __syncthreads();
+    // a thread per expert (experts <= threads)
+    if (tid < experts) {
+        int sum = 0;
+        for (int w = 0; w < kSortWarps; ++w) {
+            const int c = lines[w * experts + tid];
+            lines[w * experts + tid] = sum;
+            sum += c;
+        }
+        total[tid] = sum;
+    }
+    int all = 0, before = 0;
+    if (ctas > 1) {
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (tid < experts) {
+            const uint32_t addr = static_cast<uint32_t>(__cvta_generic_to_shared(total + tid));
+            for (int c = 0; c < ctas; ++c) {
+                uint32_t remote, v;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(c));
+                asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
+                if (c < cta) before += int(v);
+                all += int(v);
+            }
+        }
+        // no CTA leaves while another reads its counts: the other half of this barrier is at the end
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    } else if (tid < experts) {
+        all = total[tid];
+    }
+    // exclusive sums of the padded counts over the experts
+    const int padded = tid < experts ? (all + align - 1) / align * align : 0;
+    int sum = padded;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, d);
+        if (lane >= d) sum += v;
+    }
+    if (lane == 31) warp_sums[warp] = sum;
+    __syncthreads();
+    if (warp == 0) {
+        int v = warp_sums[lane];
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int u = __shfl_up_sync(0xffffffffu, v, d);
+            if (lane >= d) v += u;
+        }
+        warp_sums[lane] = v;
+    }
+    __syncthreads();
+    const int run = sum - padded + (warp > 0 ? warp_sums[warp - 1] : 0);
+    if (tid < experts) {
+        count[tid] = all;
+        start[tid] = run;
+        if (tid == experts - 1) start[experts] = run + padded;
+        for (int w = 0; w < kSortWarps; ++w) lines[w * experts + tid] += run + before;
+        if (cta == 0) {
+            offsets[tid] = run;
+            if (tid == experts - 1) offsets[experts] = run + padded;
+        }
+    }
+    __syncthreads();
+
+    for (int p0 = begin; p0 < end; p0 += 32) {
+        const int p = p0 + lane;
+        const int e = expert_of(ids, p, end, experts);
+        const uint32_t same = __match_any_sync(0xffffffffu, e);
+        int at = -1;
+        if (e >= 0) at = line[e] + __popc(same & ((1u << lane) - 1u));
+        __syncwarp();
+        if (e >= 0 && lane == 31 - __clz(same)) line[e] = at + 1;
+        __syncwarp();
+        if (p < end) rows[p] = at;
+        if (at >= 0 && at < n_rows) pairs[at] = p;
+    }
+    // the rows' experts, and the rows without a pair
+    for (int r = cta * kSortThreads + tid; r < n_rows; r += ctas * kSortThreads) {
+        int lo = 0, hi = experts;  // the last expert whose run starts at or before r (empty runs start where the next does)
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (start[mid] <= r) lo = mid; else hi = mid;
+        }
+        expert_ids[r] = lo;
+        if (r - start[lo] >= count[lo]) pairs[r] = -1;
+    }
+    __syncwarp();
+    if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// ---------------------------------------------------------------------------- tokens to rows
+//
+// A CTA reads a piece of one token and writes it to each of the token's rows; the CTAs behind the tokens zero the rows that
+// pad the experts' runs.  Unit: the widest word that the rows' starts and length allow.
+
+constexpr int kMoveThreads = 256;
+
+template <typename Unit, int kPer>
+__global__ void __launch_bounds__(kMoveThreads) moe_permute_kernel(const Unit* __restrict__ x, int64_t ld, int tokens, int units, int topk,
+                                                                   const int* __restrict__ rows, const int* __restrict__ pairs,
+                                                                   const int* __restrict__ offsets, int n_rows, Unit* __restrict__ out) {
+    grid_wait();
+    grid_launch_dependents();
+    const int c = blockIdx.y * (kMoveThreads * kPer) + threadIdx.x;
+    if (int(blockIdx.x) >= tokens) {
+        const int e = int(blockIdx.x) - tokens;
+        for (int r = min(offsets[e + 1], n_rows) - 1; r >= max(offsets[e], 0) && pairs[r] < 0; --r) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                if (c + i * kMoveThreads < units) out[int64_t(r) * units + c + i * kMoveThreads] = Unit{};
+            }
+        }
+        return;
+    }
+    const int64_t token = blockIdx.x;
+    Unit v[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        if (c + i * kMoveThreads < units) v[i] = x[token * ld + c + i * kMoveThreads];
+    }
+    for (int j = 0; j < topk; ++j) {
+        const int r = __ldg(rows + token * topk + j);
+        if (r < 0 || r >= n_rows) continue;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            if (c + i * kMoveThreads < units) out[int64_t(r) * units + c + i * kMoveThreads] = v[i];
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------- rows to tokens
+//
+// y[t] = sum over the token's slots, in their order and in float32, of weight * z[row]; rounded once.
+
+template <typename T>
+struct Floats;  // a piece of kN values in one load
+template <>
+struct Floats<__nv_bfloat16> {
+    static constexpr int kN = 8;
+    using Vec = uint4;
+    static __device__ __forceinline__ void get(const uint4& v, float (&f)[8]) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ uint4 put(const float (&f)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+            memcpy(&w[i], &h, 4);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+template <>
+struct Floats<__half> {
+    static constexpr int kN = 8;
+    using Vec = uint4;
+    static __device__ __forceinline__ void get(const uint4& v, float (&f)[8]) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            __half2 h;
+            memcpy(&h, &w[i], 4);
+            const float2 p = __half22float2(h);
+            f[2 * i] = p.x;
+            f[2 * i + 1] = p.y;
+        }
+    }
+    static __device__ __forceinline__ uint4 put(const float (&f)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+            memcpy(&w[i], &h, 4);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+template <>
+struct Floats<float> {
+    static constexpr int kN = 4;
+    using Vec = float4;
+    static __device__ __forceinline__ void get(const float4& v, float (&f)[4]) { f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w; }
+    static __device__ __forceinline__ float4 put(const float (&f)[4]) { return make_float4(f[0], f[1], f[2], f[3]); }
+};
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+// kWide: pieces of 16 bytes (all rows start on 16 bytes), else single values.  A piece at `c` of a row of `h` values.
+template <typename T, bool kWide>
+struct Piece {
+    static constexpr int kN = kWide ? Floats<T>::kN : 1;
+    using Vec = typename Floats<T>::Vec;
+    Vec v;
+    T one;
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (kWide) v = __ldg(reinterpret_cast<const Vec*>(p)); else one = p[0];
+    }
+    __device__ __forceinline__ void get(float (&f)[kN]) const {
+        if constexpr (kWide) Floats<T>::get(v, f); else f[0] = to_float(one);
+    }
+    static __device__ __forceinline__ void store(T* p, const float (&f)[kN]) {
+        if constexpr (kWide) *reinterpret_cast<Vec*>(p) = Floats<T>::put(f); else p[0] = from_float<T>(f[0]);
+    }
+};
+
+template <typename T, bool kWide>
+__global__ void __launch_bounds__(kMoveThreads) moe_unpermute_kernel(const T* __restrict__ z, int64_t ld, int tokens, int h, int topk,
+                                                                     const int* __restrict__ rows, int n_rows,
+                                                                     const float* __restrict__ weights, T* __restrict__ y) {
+    using P = Piece<T, kWide>;
+    constexpr int kSlots = 4;  // rows loaded before the first is added
+    grid_wait();
+    grid_launch_dependents();
+    const int64_t token = blockIdx.x;
+    const int c = (blockIdx.y * kMoveThreads + threadIdx.x) * P::kN;
+    if (c >= h) return;
+    float sum[P::kN];
+#pragma unroll
+    for (int i = 0; i < P::kN; ++i) sum[i] = 0.0f;
+    for (int j0 = 0; j0 < topk; j0 += kSlots) {
+        P piece[kSlots];
+        float w[kSlots];
+        bool here[kSlots];
+#pragma unroll
+        for (int j = 0; j < kSlots; ++j) {
+            int r = -1;
+            if (j0 + j < topk) r = __ldg(rows + token * topk + j0 + j);
+            here[j] = r >= 0 && r < n_rows;
+            w[j] = 1.0f;
+            if (here[j]) {
+                piece[j].load(z + int64_t(r) * ld + c);
+                if (weights != nullptr) w[j] = __ldg(weights + token * topk + j0 + j);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kSlots; ++j) {
+            if (!here[j]) continue;
+            float f[P::kN];
+            piece[j].get(f);
+#pragma unroll
+            for (int i = 0; i < P::kN; ++i) sum[i] = fmaf(w[j], f[i], sum[i]);
+        }
+    }
+    P::store(y + token * h + c, sum);
+}
+
+// The gradients of the above: gz[row] = weight * gy[token], gw[pair] = <gy[token], z[row]>.  A CTA has one token, whose
+// gradient stays in registers (up to kKeep pieces a thread, the rest is read again per slot); the CTAs behind the tokens zero the rows
+// that pad the runs.
+template <typename T, bool kWide>
+__global__ void __launch_bounds__(kMoveThreads) moe_unpermute_backward_kernel(
+    const T* __restrict__ gy, int64_t ld_g, const T* __restrict__ z, int64_t ld_z, int tokens, int h, int topk, const int* __restrict__ rows,
+    const int* __restrict__ pairs, const int* __restrict__ offsets, int n_rows, const float* __restrict__ weights, T* __restrict__ gz,
+    float* __restrict__ gw) {
+    using P = Piece<T, kWide>;
+    constexpr int kKeep = 2, kStep = kMoveThreads * P::kN;
+    __shared__ float parts[2][kMoveThreads / 32];
+    grid_wait();
+    grid_launch_dependents();
+    const int c0 = threadIdx.x * P::kN;
+    if (int(blockIdx.x) >= tokens) {
+        const int e = int(blockIdx.x) - tokens;
+        float zero[P::kN];
+#pragma unroll
+        for (int i = 0; i < P::kN; ++i) zero[i] = 0.0f;
+        for (int r = min(offsets[e + 1], n_rows) - 1; r >= max(offsets[e], 0) && pairs[r] < 0; --r) {
+            for (int c = c0; c < h; c += kStep) P::store(gz + int64_t(r) * h + c, zero);
+        }
+        return;
+    }
+    const int64_t token = blockIdx.x;
+    const T* const g = gy + token * ld_g;
+    P kept[kKeep];
+#pragma unroll
+    for (int i = 0; i < kKeep; ++i) {
+        if (c0 + i * kStep < h) kept[i].load(g + c0 + i * kStep);
+    }
+    for (int j = 0; j < topk; ++j) {
+        const int r = __ldg(rows + token * topk + j);  // the same for the whole CTA
+        if (r < 0 || r >= n_rows) {
+            if (gw != nullptr && threadIdx.x == 0) gw[token * topk + j] = 0.0f;
+            continue;
+        }
+        const float w = weights != nullptr ? __ldg(weights + token * topk + j) : 1.0f;
+        float dot = 0.0f;
+        const auto piece = [&](const P& p, int c) {
+            float f[P::kN], o[P::kN];
+            p.get(f);
+#pragma unroll
+            for (int i = 0; i < P::kN; ++i) o[i] = w * f[i];
+            if (gw != nullptr) {
+                P s;
+                s.load(z + int64_t(r) * ld_z + c);
+                float u[P::kN];
+                s.get(u);
+#pragma unroll
+                for (int i = 0; i < P::kN; ++i) dot = fmaf(f[i], u[i], dot);
+            }
+            P::store(gz + int64_t(r) * h + c, o);
+        };
+#pragma unroll
+        for (int i = 0; i < kKeep; ++i) {
+            if (c0 + i * kStep < h) piece(kept[i], c0 + i * kStep);
+        }
+        for (int c = c0 + kKeep * kStep; c < h; c += kStep) {
+            P p;
+            p.load(g + c);
+            piece(p, c);
+        }
+        if (gw != nullptr) {
+#pragma unroll
+            for (int d = 16; d > 0; d /= 2) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+            // two sets of sums, used in turn: a set is written again only behind the next slot's barrier
+            if ((threadIdx.x & 31) == 0) parts[j & 1][threadIdx.x >> 5] = dot;
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kMoveThreads / 32; ++i) sum += parts[j & 1][i];
+                gw[token * topk + j] = sum;
+            }
+        }
+    }
+}
+
+struct SortOptIn {
+    std::mutex mu;
+    int done[64] = {};
+};
+
+template <typename Id>
+cudaError_t launch_sort(const void* ids, int pairs_n, int experts, int align, int n_rows, bool pdl, int* rows, int* pairs, int* offsets,
+                        int* expert_ids, cudaStream_t stream) {
+    static SortOptIn opt;
+    // One CTA goes over 128 pairs a warp in 4 steps; from there on 8 CTAs repay the two barriers of their cluster.
+    const int ctas = pairs_n > 4096 || n_rows > 16384 ? 8 : 1;
+    const int bytes = int(sizeof(int)) * ((kSortWarps + 3) * experts + 1);
+    if (bytes > 40 * 1024) {
+        int dev = 0;
+        const cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        const std::lock_guard<std::mutex> lock(opt.mu);
+        if (dev < 0 || dev >= 64 || opt.done[dev] == 0) {
+            const int most = int(sizeof(int)) * ((kSortWarps + 3) * kMaxExperts + 1);
+            const cudaError_t f = cudaFuncSetAttribute(moe_sort_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+            if (f != cudaSuccess) return f;
+            if (dev >= 0 && dev < 64) opt.done[dev] = 1;
+        }
+    }
+    return launch(moe_sort_kernel<Id>, dim3(ctas), dim3(kSortThreads), size_t(bytes), stream, pdl, unsigned(ctas), static_cast<const Id*>(ids),
+                  pairs_n, experts, align, n_rows, ctas, rows, pairs, offsets, expert_ids);
+}
+
+template <typename Unit>
+cudaError_t launch_permute(const void* x, int64_t ld_bytes, int64_t tokens, int64_t row_bytes, int topk, const int* rows, const int* pairs,
+                           const int* offsets, int64_t experts, int n_rows, void* out, bool pdl, cudaStream_t stream) {
+    constexpr int kPer = sizeof(Unit) == 16 ? 2 : 4;
+    const int units = int(row_bytes / int64_t(sizeof(Unit)));
+    const dim3 grid(unsigned(tokens + experts), unsigned((units + kMoveThreads * kPer - 1) / (kMoveThreads * kPer)));
+    return launch(moe_permute_kernel<Unit, kPer>, grid, dim3(kMoveThreads), 0, stream, pdl, 1, static_cast<const Unit*>(x),
+                  ld_bytes / int64_t(sizeof(Unit)), int(tokens), units, topk, rows, pairs, offsets, n_rows, static_cast<Unit*>(out));
+}
+
+// What the calls on tokens and rows have in common.
+int check_moe(int64_t tokens, int64_t topk, int64_t n_rows, int64_t experts, char* err, size_t errlen) {
+    if (tokens < 0 || topk < 0 || n_rows < 0 || experts < 0 || tokens > INT32_MAX || topk > INT32_MAX || n_rows > INT32_MAX ||
+        tokens * topk > INT32_MAX || experts > kMaxExperts || tokens + experts > INT32_MAX) {
+        return fail(err, errlen, HQ_ERR_INVALID, "at most 2^31 - 1 pairs and rows and %d experts, got %lld tokens of %lld, %lld rows, %lld experts",
+                    kMaxExperts, static_cast<long long>(tokens), static_cast<long long>(topk), static_cast<long long>(n_rows),
+                    static_cast<long long>(experts));
+    }
+    return HQ_OK;
+}
+
+int element_size(int dtype) { return dtype == HQ_DTYPE_FP32 ? 4 : dtype == HQ_DTYPE_BF16 || dtype == HQ_DTYPE_FP16 ? 2 : 0; }
+
+}  // namespace
+}  // namespace hq
+
+extern "C" int hq_moe_sort(const void* ids, int ids_bytes, int64_t tokens, int64_t topk, int64_t num_experts, int64_t align, int64_t n_rows,
+                           int use_pdl, int32_t* rows, int32_t* pairs, int32_t* offsets, int32_t* expert_ids, int device, void* stream,
+                           char* err, size_t errlen) {
+    using hq::fail;
+    if (ids_bytes != 4 && ids_bytes != 8) return fail(err, errlen, HQ_ERR_INVALID, "topk_ids must be int32 or int64");
+    if (num_experts < 1) return fail(err, errlen, HQ_ERR_INVALID, "num_experts must be at least 1, got %lld", static_cast<long long>(num_experts));
+    const int rc = hq::check_moe(tokens, topk, n_rows, num_experts, err, errlen);
+    if (rc != HQ_OK) return rc;
+    if (align < 1 || align > 65536) return fail(err, errlen, HQ_ERR_INVALID, "align must be in [1, 65536], got %lld", static_cast<long long>(align));
+    // any ids have to fit: what pads the runs of as many experts as there can be
+    const int64_t n = tokens * topk, need = (n + (n < num_experts ? n : num_experts) * (align - 1)) / align * align;
+    if (n_rows < need) {
+        return fail(err, errlen, HQ_ERR_INVALID, "%lld rows are needed for %lld pairs, %lld experts and runs on multiples of %lld, got %lld",
+                    static_cast<long long>(need), static_cast<long long>(n), static_cast<long long>(num_experts), static_cast<long long>(align),
+                    static_cast<long long>(n_rows));
+    }
+    if (offsets == nullptr || (n > 0 && (ids == nullptr || rows == nullptr)) || (n_rows > 0 && (pairs == nullptr || expert_ids == nullptr))) {
+        return fail(err, errlen, HQ_ERR_INVALID, "null pointer argument");
+    }
+    const hq::DeviceGuard guard(device);
+    if (!guard.ok()) return fail(err, errlen, HQ_ERR_CUDA, "cannot select CUDA device %d", device);
+    const auto s = static_cast<cudaStream_t>(stream);
+    HQ_CUDA_TRY(ids_bytes == 8 ? hq::launch_sort<int64_t>(ids, int(n), int(num_experts), int(align), int(n_rows), use_pdl != 0, rows, pairs,
+                                                          offsets, expert_ids, s)
+                               : hq::launch_sort<int32_t>(ids, int(n), int(num_experts), int(align), int(n_rows), use_pdl != 0, rows, pairs,
+                                                          offsets, expert_ids, s));
+    return HQ_OK;
+}
+
+extern "C" int hq_moe_permute(const void* input, int64_t ld_bytes, int64_t tokens, int64_t row_bytes, int64_t topk, const int32_t* rows,
+                              const int32_t* pairs, const int32_t* offsets, int64_t num_experts, int64_t n_rows, int padded, int use_pdl,
+                              void* output, int device, void* stream, char* err, size_t errlen) {
+    using hq::fail;
+    const int rc = hq::check_moe(tokens, topk, n_rows, num_experts, err, errlen);
+    if (rc != HQ_OK) return rc;
+    if (row_bytes < 0 || row_bytes > (int64_t(1) << 24)) return fail(err, errlen, HQ_ERR_INVALID, "rows of at most 16 MiB");
+    if (tokens == 0 || topk == 0 || row_bytes == 0) return HQ_OK;  // no pairs, no runs
+    if (input == nullptr || rows == nullptr || pairs == nullptr || offsets == nullptr || output == nullptr) {
+        return fail(err, errlen, HQ_ERR_INVALID, "null pointer argument");
+    }
+    const hq::DeviceGuard guard(device);
+    if (!guard.ok()) return fail(err, errlen, HQ_ERR_CUDA, "cannot select CUDA device %d", device);
+    const auto s = static_cast<cudaStream_t>(stream);
+    const auto fits = [&](size_t a) {
+        return hq::aligned(input, a) && hq::aligned(output, a) && ld_bytes % int64_t(a) == 0 && row_bytes % int64_t(a) == 0;
+    };
+    const auto go = [&](auto unit) {
+        return hq::launch_permute<decltype(unit)>(input, ld_bytes, tokens, row_bytes, int(topk), rows, pairs, offsets,
+                                                  padded != 0 ? num_experts : 0, int(n_rows), output, use_pdl != 0, s);
+    };
+    HQ_CUDA_TRY(fits(16) ? go(uint4{}) : fits(4) ? go(uint32_t{}) : fits(2) ? go(uint16_t{}) : go(uint8_t{}));
+    return HQ_OK;
+}
+
+extern "C" int hq_moe_unpermute(const void* input, int64_t ld_elems, int dtype, int64_t n_rows, int64_t h, int64_t tokens, int64_t topk,
+                                const int32_t* rows, const float* weights, int use_pdl, void* output, int device, void* stream, char* err,
+                                size_t errlen) {
+    using hq::fail;
+    const int rc = hq::check_moe(tokens, topk, n_rows, 0, err, errlen);
+    if (rc != HQ_OK) return rc;
+    const int size = hq::element_size(dtype);
+    if (size == 0) return fail(err, errlen, HQ_ERR_INVALID, "input dtype must be bfloat16, float16 or float32");
+    if (h < 0 || h > (int64_t(1) << 22)) return fail(err, errlen, HQ_ERR_INVALID, "hidden size must be at most 2^22");
+    if (tokens == 0 || h == 0) return HQ_OK;
+    if (output == nullptr || (topk > 0 && rows == nullptr) || (n_rows > 0 && input == nullptr)) {
+        return fail(err, errlen, HQ_ERR_INVALID, "null pointer argument");
+    }
+    const hq::DeviceGuard guard(device);
+    if (!guard.ok()) return fail(err, errlen, HQ_ERR_CUDA, "cannot select CUDA device %d", device);
+    const bool wide = hq::aligned(input, 16) && hq::aligned(output, 16) && ld_elems * size % 16 == 0 && h * size % 16 == 0;
+    const int64_t per = hq::kMoveThreads * int64_t(wide ? 16 / size : 1);
+    const dim3 grid(unsigned(tokens), unsigned((h + per - 1) / per));
+    const auto go = [&](auto kernel, auto* z) {
+        using T = std::remove_const_t<std::remove_pointer_t<decltype(z)>>;
+        return hq::launch(kernel, grid, dim3(hq::kMoveThreads), 0, static_cast<cudaStream_t>(stream), use_pdl != 0, 1, z, ld_elems, int(tokens),
+                          int(h), int(topk), rows, int(n_rows), weights, static_cast<T*>(output));
+    };
+    const auto typed = [&](auto* z) {
+        using T = std::remove_const_t<std::remove_pointer_t<decltype(z)>>;
+        return wide ? go(hq::moe_unpermute_kernel<T, true>, z) : go(hq::moe_unpermute_kernel<T, false>, z);
+    };
+    HQ_CUDA_TRY(dtype == HQ_DTYPE_BF16   ? typed(static_cast<const __nv_bfloat16*>(input))
+                : dtype == HQ_DTYPE_FP16 ? typed(static_cast<const __half*>(input))
+                                         : typed(static_cast<const float*>(input)));
+    return HQ_OK;
+}
+
+extern "C" int hq_moe_unpermute_backward(const void* grad_output, int64_t ld_grad, const void* input, int64_t ld_input, int dtype, int64_t n_rows,
+                                         int64_t h, int64_t tokens, int64_t topk, const int32_t* rows, const int32_t* pairs,
+                                         const int32_t* offsets, int64_t num_experts, int padded, const float* weights, int use_pdl,
+                                         void* grad_input, float* grad_weights, int device, void* stream, char* err, size_t errlen) {
+    using hq::fail;
+    const int rc = hq::check_moe(tokens, topk, n_rows, num_experts, err, errlen);
+    if (rc != HQ_OK) return rc;
+    const int size = hq::element_size(dtype);
+    if (size == 0) return fail(err, errlen, HQ_ERR_INVALID, "input dtype must be bfloat16, float16 or float32");
+    if (h < 0 || h > (int64_t(1) << 22)) return fail(err, errlen, HQ_ERR_INVALID, "hidden size must be at most 2^22");
+    if (tokens == 0 || topk == 0) return HQ_OK;
+    if ((h > 0 && (grad_output == nullptr || grad_input == nullptr || (grad_weights != nullptr && input == nullptr))) || rows == nullptr ||
+        pairs == nullptr || offsets == nullptr) {
+        return fail(err, errlen, HQ_ERR_INVALID, "null pointer argument");
+    }
+    const hq::DeviceGuard guard(device);
+    if (!guard.ok()) return fail(err, errlen, HQ_ERR_CUDA, "cannot select CUDA device %d", device);
+    const bool wide = hq::aligned(grad_output, 16) && hq::aligned(grad_input, 16) && hq::aligned(input, 16) && ld_grad * size % 16 == 0 &&
+                      ld_input * size % 16 == 0 && h * size % 16 == 0;
+    const dim3 grid(unsigned(tokens + (padded != 0 ? num_experts : 0)));
+    const auto go = [&](auto kernel, auto* g) {
+        using T = std::remove_const_t<std::remove_pointer_t<decltype(g)>>;
+        return hq::launch(kernel, grid, dim3(hq::kMoveThreads), 0, static_cast<cudaStream_t>(stream), use_pdl != 0, 1, g, ld_grad,
+                          static_cast<const T*>(input), ld_input, int(tokens), int(h), int(topk), rows, pairs, offsets, int(n_rows), weights,
+                          static_cast<T*>(grad_input), grad_weights);
+    };
+    const auto typed = [&](auto* g) {
+        using T = std::remove_const_t<std::remove_pointer_t<decltype(g)>>;
+        return wide ? go(hq::moe_unpermute_backward_kernel<T, true>, g) : go(hq::moe_unpermute_backward_kernel<T, false>, g);
+    };
+    HQ_CUDA_TRY(dtype == HQ_DTYPE_BF16   ? typed(static_cast<const __nv_bfloat16*>(grad_output))
+                : dtype == HQ_DTYPE_FP16 ? typed(static_cast<const __half*>(grad_output))
+                                         : typed(static_cast<const float*>(grad_output)));
+    return HQ_OK;
+}

@@ -33,8 +33,9 @@ enum {
     HQ_MODE_W4A8_MXFP4 = 3
 };
 
-/* Input element type of the quantizer. */
-enum { HQ_DTYPE_BF16 = 0, HQ_DTYPE_FP16 = 1 };
+/* Element types: inputs of the quantizers (BF16, FP16), outputs of the block-128 products and tokens
+ * of the hq_moe_* calls (all three). */
+enum { HQ_DTYPE_BF16 = 0, HQ_DTYPE_FP16 = 1, HQ_DTYPE_FP32 = 2 };
 
 /* Epilogue selector; values of the reference's EpilogueOp
  * (csrc/kernel/gemm/epilogue_op.h:21-28).  hq_dense_gemm takes Identity and Sigmoid,
@@ -295,6 +296,100 @@ int hq_sm_count(int device);
  * the environment is changed (CPython's interpreter lock), and gives it up for the call, reads them itself before it
  * does: hold != 0 reads them now, and the calls of this thread take that reading until hold == 0. */
 void hq_hold_switches(int hold);
+
+/*
+ * FP8 with a float32 scale per block of 128 (no counterpart in the reference).
+ *
+ * Quantisation: over every block amax = max(max |x|, 1e-10), scale = amax / 448, code = e4m3(x * 448 / amax), nearest,
+ * ties to even; a NaN or an infinity makes its block's scale NaN or infinite.
+ *   input       `batches` matrices [m, k] bf16 / fp16, `ld_elems` between rows and `batch_stride` elements between
+ *               matrices; rows 16-byte aligned, k a multiple of 16
+ *   block_rows  1: blocks of 1 x 128 along k (one matrix); 128: blocks of 128 x 128
+ *   transpose   0: out_q [batches, m, k], out_sf [m, ceil(k/128)] or [batches, ceil(m/128), ceil(k/128)];
+ *               1: of the transposed matrices: out_q [batches, k, ceil(m/16)*16], columns from m on zero,
+ *               out_sf [k, ceil(m/128)] (block_rows 1: blocks of 128 along m) or [batches, ceil(k/128), ceil(m/128)]
+ */
+int hq_block_quant(const void* input, int64_t ld_elems, int64_t batch_stride, int in_dtype, int64_t batches, int64_t m,
+                   int64_t k, int block_rows, int transpose, int use_pdl, void* out_q, void* out_sf, int device,
+                   void* stream, char* err, size_t errlen);
+
+/*
+ * h = silu(gate) * up in float32 for rows [gate | up] of 2k values, quantised in blocks of 1 x 128 as hq_block_quant does.
+ *   input      [m, 2k] bf16 / fp16, rows 16-byte aligned, k a multiple of 16
+ *   row_limit  NULL, or device pointer to one int: rows from there on are neither read nor written
+ *   out_q      [m, k] e4m3, out_sf [m, ceil(k/128)] float32
+ */
+int hq_swiglu_block_quant(const void* input, int64_t ld_elems, int in_dtype, int64_t m, int64_t k,
+                          const int32_t* row_limit, int use_pdl, void* out_q, void* out_sf, int device, void* stream,
+                          char* err, size_t errlen);
+
+/*
+ * out[M, N] = sum over blocks b of K of sfa[m, b] * sfb[n / 128, b] * (a[m, b] . b[n, b]), summed in float32 and rounded once.
+ *   a, b        [M, K], [N, K] e4m3, row-major contiguous, 16-byte aligned; K a multiple of 16 (a last block may be short)
+ *   sfa         [M, ceil(K/128)] float32
+ *   sfb         [ceil(N/128), ceil(K/128)] float32, or with row_scales != 0 [N, ceil(K/128)] (one per row of b)
+ *   out         [M, N] of out_dtype (HQ_DTYPE_*), `ldo` elements between rows
+ */
+int hq_block_gemm(const void* a, const void* b, const float* sfa, const float* sfb, void* out, int out_dtype, int64_t m,
+                  int64_t n, int64_t k, int row_scales, int64_t ldo, int sm_count, int use_pdl, int device, void* stream,
+                  char* err, size_t errlen);
+
+/*
+ * The same for rows in runs of one expert: rows [offsets[e], offsets[e + 1]) of a times b[e], others are not written.
+ *   b        [num_experts, N, K] e4m3, sfb [num_experts, ceil(N/128), ceil(K/128)]; at most 1024 experts
+ *   offsets  [num_experts + 1] non-decreasing row numbers on the device; runs may start anywhere (one that goes back or lies
+ *            outside of [0, M] is clamped)
+ */
+int hq_group_block_gemm(const void* a, const void* b, const float* sfa, const float* sfb, const int32_t* offsets,
+                        void* out, int out_dtype, int64_t num_experts, int64_t m, int64_t n, int64_t k, int64_t ldo,
+                        int sm_count, int use_pdl, int device, void* stream, char* err, size_t errlen);
+
+/*
+ * Tokens in the order of the experts that a router gave them, and back (no counterpart in the reference).
+ *
+ * hq_moe_sort: pair p = token * topk + slot has expert ids[p] (int32 or int64, ids_bytes 4 or 8); one outside of
+ * [0, num_experts) is dropped.  The pairs of an expert keep their order; its run of rows starts on a multiple of `align`.
+ *   rows        [tokens, topk]     the pair's row, -1 for a dropped one
+ *   pairs       [n_rows]           the row's pair, -1 where there is none
+ *   offsets     [num_experts + 1]  first row of each run, and the end of the last (padding included)
+ *   expert_ids  [n_rows]           the run that a row is in, num_experts - 1 behind the last
+ * n_rows is at least floor((p + min(num_experts, p) * (align - 1)) / align) * align for p pairs.
+ */
+int hq_moe_sort(const void* ids, int ids_bytes, int64_t tokens, int64_t topk, int64_t num_experts, int64_t align,
+                int64_t n_rows, int use_pdl, int32_t* rows, int32_t* pairs, int32_t* offsets, int32_t* expert_ids,
+                int device, void* stream, char* err, size_t errlen);
+
+/*
+ * output[row] = input[token of the row's pair]; with `padded` != 0 rows without a pair inside of the runs are zeroed.  Rows behind
+ * the last run are not written.  Rows are `row_bytes` long (output rows follow one another), `ld_bytes` apart in the input.
+ */
+int hq_moe_permute(const void* input, int64_t ld_bytes, int64_t tokens, int64_t row_bytes, int64_t topk,
+                   const int32_t* rows, const int32_t* pairs, const int32_t* offsets, int64_t num_experts, int64_t n_rows,
+                   int padded, int use_pdl, void* output, int device, void* stream, char* err, size_t errlen);
+
+/* The same of [tokens, k] bf16 / fp16, quantised on the way as hq_block_quant does (rows that pad a run: as zeros). */
+int hq_moe_permute_block_quant(const void* input, int64_t ld_elems, int in_dtype, int64_t tokens, int64_t k, int64_t topk,
+                               const int32_t* rows, const int32_t* pairs, const int32_t* offsets, int64_t num_experts,
+                               int64_t n_rows, int padded, int use_pdl, void* out_q, void* out_sf, int device,
+                               void* stream, char* err, size_t errlen);
+
+/*
+ * output[t] = sum over the token's slots of weights[t, s] * input[rows[t, s]] in float32, in the slots' order, rounded
+ * once; slots without a row are left out, weights NULL counts as ones.  With weights NULL it is the gradient of hq_moe_permute.
+ */
+int hq_moe_unpermute(const void* input, int64_t ld_elems, int dtype, int64_t n_rows, int64_t h, int64_t tokens,
+                     int64_t topk, const int32_t* rows, const float* weights, int use_pdl, void* output, int device,
+                     void* stream, char* err, size_t errlen);
+
+/*
+ * The gradients of hq_moe_unpermute: grad_input[row] = weights[pair] * grad_output[token] (rows as hq_moe_permute writes
+ * them), grad_weights[t, s] = <grad_output[t], input[row]> in float32, 0 for a slot without a row; NULL if not wanted.
+ */
+int hq_moe_unpermute_backward(const void* grad_output, int64_t ld_grad, const void* input, int64_t ld_input, int dtype,
+                              int64_t n_rows, int64_t h, int64_t tokens, int64_t topk, const int32_t* rows,
+                              const int32_t* pairs, const int32_t* offsets, int64_t num_experts, int padded,
+                              const float* weights, int use_pdl, void* grad_input, float* grad_weights, int device,
+                              void* stream, char* err, size_t errlen);
 
 /*
  * Reads (and clears) the device-side status word of `device` after
