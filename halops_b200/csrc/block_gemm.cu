@@ -10,8 +10,8 @@
 //   warps 0-7  promotion: tcgen05.ld of a block's sums, accumulators += scale * sums (two columns an instruction); after the last
 //              block the accumulators are rounded once and stored.  A thread has one row and half of the tile's columns.
 //   warp 8     TMA producer: A and B tiles (128-byte swizzle) into a ring of stages
-//   warp 9     issues the MMAs of a block into the next of 2 (BN = 256) or 4 buffers of tensor memory
-//   warp 10    (a scale per row of the second operand) brings the scales of a block into shared memory
+//   warps 9, 11  issue the MMAs of a block into the next of 2 (BN = 256) or 4 buffers of tensor memory, every other block each
+//   warp 10    brings the scales of four blocks at a time into shared memory, multiplied where a row has one factor per block
 //
 // Every mbarrier wait is bounded, as in the other GEMM kernels: a role that waits longer than kTimeoutNs records a code in the
 // status word, raises the CTA's abort flag and all roles leave through the common teardown.
@@ -30,10 +30,13 @@ namespace {
 
 constexpr int kTileM = 128;
 constexpr int kBlockK = 128;  // values, and bytes, of a k-tile row
-constexpr int kPromoWarps = 8;
+constexpr int kParts = 2;  // groups of four warps that share a tile's columns
+constexpr int kPromoWarps = 4 * kParts;
+constexpr int kLoadWarp = kPromoWarps, kScaleWarp = kPromoWarps + 1, kMmaWarp = kPromoWarps + 2;  // and kMmaWarp + 1
 constexpr int kMaxExperts = 1024;
 constexpr int kSmemBudget = 232448;
-constexpr int kScaleSlots = 4;
+constexpr int kGroupK = 4;      // k-tiles whose scales are brought together
+constexpr int kScaleSlots = 2;  // such groups in shared memory
 
 struct BlockBars {
     uint64_t full[8];
@@ -53,17 +56,21 @@ struct BlockCfg {
     static constexpr int kStageBytes = kABytes + kBBytes;
     static constexpr int kBarBytes = 512;
     static constexpr int kTableBytes = (kMaxExperts + 8) * 8;                // grouped: row tiles before, first row of, each expert
-    static constexpr int kScaleBytes = kRowScales ? kScaleSlots * BN * 4 : 0;
+    static constexpr int kWeightBlocks = kRowScales ? 1 : (BN + 127) / 128;  // blocks of 128 weight rows that a tile spans
+    // a k-tile's scales: per row of the tile one for each of its blocks of weights (the product of both), or (kRowScales) the rows' and then the columns'
+    static constexpr int kScales = kRowScales ? kTileM + BN : kTileM * kWeightBlocks;
+    static constexpr int kScaleBytes = kScaleSlots * kGroupK * kScales * 4;
     static constexpr int kExtra = kBarBytes + kTableBytes + kScaleBytes + 1024;
     static constexpr int kFit = (kSmemBudget - kExtra) / kStageBytes;
     static constexpr int kStages = kFit > 8 ? 8 : kFit;
     static constexpr int kSmemBytes = kStages * kStageBytes + kExtra;
     static constexpr int kBufs = BN == 256 ? 2 : 4;
     static constexpr int kTmemCols = kBufs * BN;
-    static constexpr int kCols = BN / 2;  // columns of a promotion warp
-    // BN = 256: 128 accumulators a thread; the third warpgroup gives registers to the other two (168 * 384 = 232 * 256 + 40 * 128)
+    static constexpr int kCols = BN / kParts;  // columns of a promotion warp
+    static constexpr int kLd = BN == 256 ? 16 : kCols < 32 ? kCols : 32;  // of which one load brings
+    static constexpr int kThreads = (kPromoWarps + 4) * 32;
+    // BN = 256: 128 accumulators a thread; the third warpgroup gives registers to the other two (168 * 384 = 208 * 256 + 88 * 128)
     static constexpr bool kRegSplit = BN == 256;
-    static constexpr int kThreads = kRegSplit ? 384 : (kPromoWarps + 2 + (kRowScales ? 1 : 0)) * 32;
     static_assert(sizeof(BlockBars) <= kBarBytes && kStages >= 3 && kTmemCols <= 512, "budgets");
     static_assert(kTileM * (BN + 4) * 4 <= kStages * kStageBytes, "split-K partial sums fit into the ring");
 };
@@ -81,6 +88,7 @@ struct BlockArgs {
     int out_type;   // HQ_DTYPE_*
     int out_align;  // 32, 16 or less: bytes that every row of the output starts on
     int split;      // CTAs of a cluster that share a tile's k-tiles
+    int wide_scales;  // both operands' scales are on 16 bytes
     int pdl;
 };
 
@@ -146,14 +154,24 @@ __device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t adesc, uint64_t bd
         : "memory");
 }
 
-// 32 lanes x 16 columns; the values are there behind load_wait on the same registers.
-__device__ __forceinline__ void load_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+// 32 lanes x 32 or 16 columns; the values are there behind load_wait on the same registers.
+__device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&r)[32]) { ptx::tc_load_32x32(taddr, r); }
+__device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
           "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr)
         : "memory");
+}
+__device__ __forceinline__ void load_wait(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                   "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                   "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
 }
 __device__ __forceinline__ void load_wait(uint32_t (&r)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -163,23 +181,31 @@ __device__ __forceinline__ void load_wait(uint32_t (&r)[16]) {
                  : "memory");
 }
 
-__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-    return r;
+// (a, b) += (x, y) * s as one packed instruction.  It needs the issue slots of two scalar ones, but not their operand reads: 128 columns
+// of 8 warps, loads included, take 292 cycles with it and 421 with fmaf.
+__device__ __forceinline__ void add_scaled2(float& a, float& b, uint32_t x, uint32_t y, float s) {
+    asm("{\n\t"
+        ".reg .b64 v, f, c;\n\t"
+        "mov.b64 v, {%2, %3};\n\t"
+        "mov.b64 f, {%4, %4};\n\t"
+        "mov.b64 c, {%0, %1};\n\t"
+        "fma.rn.f32x2 c, v, f, c;\n\t"
+        "mov.b64 {%0, %1}, c;\n\t"
+        "}"
+        : "+f"(a), "+f"(b)
+        : "r"(x), "r"(y), "f"(s));
 }
-__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
+// (x, y) *= (s, t)
+__device__ __forceinline__ void scale2(uint32_t& x, uint32_t& y, float s, float t) {
+    asm("{\n\t"
+        ".reg .b64 v, f;\n\t"
+        "mov.b64 v, {%0, %1};\n\t"
+        "mov.b64 f, {%2, %3};\n\t"
+        "mul.rn.f32x2 v, v, f;\n\t"
+        "mov.b64 {%0, %1}, v;\n\t"
+        "}"
+        : "+r"(x), "+r"(y)
+        : "f"(s), "f"(t));
 }
 
 __device__ __forceinline__ uint32_t pack16(float lo, float hi, int type) {
@@ -273,7 +299,7 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         ptx::prefetch_tmap(&tm_a);
         ptx::prefetch_tmap(&tm_b);
     }
-    if (warp == 9) {
+    if (warp == kMmaWarp) {
         ptx::tmem_alloc<1>(ptx::smem_u32(&bars->tmem_base), C::kTmemCols);
         ptx::tmem_relinquish<1>();
     }
@@ -324,8 +350,8 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     const int k_end = kSplit ? int(int64_t(p.k_tiles) * (rank + 1) / p.split) : p.k_tiles;
 
     if (warp >= kPromoWarps) {
-    if constexpr (C::kRegSplit) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    if (warp == 8) {
+    if constexpr (C::kRegSplit) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == kLoadWarp) {
         // ------------------------------------------------------------ TMA producer
         uint32_t it = 0;
         bool ok = true;
@@ -350,16 +376,19 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
             }
         }
         ptx::pdl_launch_dependents();
-    } else if (warp == 9) {
-        // ------------------------------------------------------------ MMA issuer
+    } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
+        // ------------------------------------------------------------ MMA issuers
+        // Every other k-tile each: every k-tile has a buffer of its own, so that nothing has to be kept in order between them.
         // float32 sums, e4m3 operands, both K-major; N >> 3, M >> 4
         constexpr uint32_t idesc = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(kTileM >> 4) << 24);
+        const uint32_t mine = warp == kMmaWarp ? 0u : 1u;
         uint32_t it = 0;
         bool ok = true;
         BlockWalk<BN, kGrouped> walk(p, tables, first, step);
         BlockTile t;
         while (ok && walk.next(t)) {
             for (int kt = k_begin; kt < k_end; ++kt, ++it) {
+                if ((it & 1u) != mine) continue;
                 const uint32_t s = it % C::kStages, buf = it % C::kBufs;
                 ok = wait_bars<true>(ptx::smem_u32(&bars->full[s]), (it / C::kStages) & 1u, true, ptx::smem_u32(&bars->acc_empty[buf]),
                                ((it / C::kBufs) & 1u) ^ 1u, abort, kStatusMma);
@@ -377,144 +406,147 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
                 if (ptx::elect_one()) ptx::tc_commit(ptx::smem_u32(&bars->empty[s]));
             }
         }
-    } else if (kRowScales && warp == 10) {
-        // ------------------------------------------------------------ scales of the second operand's rows
-        // four k-tiles are in registers before the slots are free
-        uint32_t it = 0;
+    } else if (warp == kScaleWarp) {
+        // ------------------------------------------------------------ scales
+        // A group's are in registers before its slot is free.  A lane has every 32nd row; four neighbouring k-tiles are one load where
+        // they lie on 16 bytes.
+        constexpr int kRowsA = kTileM / 32, kRowsB = kRowScales ? BN / 32 : 1;
+        const bool wide = p.k_tiles % 4 == 0 && p.wide_scales != 0;
+        const auto load4 = [&](const float* q, int k0, float (&v)[kGroupK]) {
+            if (wide && k0 % 4 == 0 && k0 + kGroupK <= k_end) {
+                const float4 f = __ldg(reinterpret_cast<const float4*>(q + k0));
+                v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+            } else {
+#pragma unroll
+                for (int i = 0; i < kGroupK; ++i) v[i] = k0 + i < k_end ? __ldg(q + k0 + i) : 0.0f;
+            }
+        };
+        uint32_t group = 0;
         bool ok = true;
         BlockWalk<BN, kGrouped> walk(p, tables, first, step);
         BlockTile t;
         while (ok && walk.next(t)) {
-            for (int k0 = k_begin; ok && k0 < k_end; k0 += kScaleSlots) {
-                float v[kScaleSlots][BN / 32];
+            const float* const pa = p.sfa + int64_t(t.row0) * p.k_tiles;
+            const int n_block = t.n0 / 128;
+            for (int k0 = k_begin; k0 < k_end; k0 += kGroupK, ++group) {
+                float a[kRowsA][kGroupK], b[kRowScales ? kRowsB : C::kWeightBlocks][kGroupK];
 #pragma unroll
-                for (int i = 0; i < kScaleSlots; ++i) {
+                for (int j = 0; j < kRowsA; ++j) load4(pa + int64_t(min(j * 32 + lane, t.valid - 1)) * p.k_tiles, k0, a[j]);
+                if constexpr (kRowScales) {
 #pragma unroll
-                    for (int j = 0; j < BN / 32; ++j) {
-                        const int n = t.n0 + j * 32 + lane;
-                        v[i][j] = k0 + i < k_end && n < p.n ? __ldg(p.sfb + (int64_t(t.expert) * p.n + n) * p.k_tiles + k0 + i) : 0.0f;
+                    for (int j = 0; j < kRowsB; ++j) load4(p.sfb + int64_t(min(t.n0 + j * 32 + lane, p.n - 1)) * p.k_tiles, k0, b[j]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < C::kWeightBlocks; ++j) {
+                        load4(p.sfb + (int64_t(t.expert) * p.n_blocks + min(n_block + j, p.n_blocks - 1)) * p.k_tiles, k0, b[j]);
                     }
                 }
+                const uint32_t slot = group % kScaleSlots;
+                ok = wait_bar<true>(ptx::smem_u32(&bars->sf_empty[slot]), ((group / kScaleSlots) & 1u) ^ 1u, abort, kStatusProducer);
+                if (!ok) break;
+                float* const to = scales + slot * (kGroupK * C::kScales) + lane;
 #pragma unroll
-                for (int i = 0; i < kScaleSlots; ++i) {
-                    if (k0 + i >= k_end) break;
-                    const uint32_t slot = it % kScaleSlots;
-                    ok = wait_bar<true>(ptx::smem_u32(&bars->sf_empty[slot]), ((it / kScaleSlots) & 1u) ^ 1u, abort, kStatusProducer);
-                    if (!ok) break;
+                for (int i = 0; i < kGroupK; ++i) {
 #pragma unroll
-                    for (int j = 0; j < BN / 32; ++j) scales[slot * BN + j * 32 + lane] = v[i][j];
-                    __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&bars->sf_full[slot]));
-                    ++it;
+                    for (int j = 0; j < kRowsA; ++j) {
+                        if constexpr (kRowScales) {
+                            to[i * C::kScales + j * 32] = a[j][i];
+                        } else {
+#pragma unroll
+                            for (int h = 0; h < C::kWeightBlocks; ++h) to[i * C::kScales + h * kTileM + j * 32] = a[j][i] * b[h][i];
+                        }
+                    }
+                    if constexpr (kRowScales) {
+#pragma unroll
+                        for (int j = 0; j < kRowsB; ++j) to[i * C::kScales + kTileM + j * 32] = b[j][i];
+                    }
                 }
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&bars->sf_full[slot]));
             }
         }
     }
     } else {
         // ------------------------------------------------------------ promotion and epilogue
-        if constexpr (C::kRegSplit) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
-        const int quarter = warp & 3, half = warp >> 2;  // lanes of tensor memory, columns
+        if constexpr (C::kRegSplit) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int quarter = warp & 3, part = warp >> 2;  // lanes of tensor memory, columns
         const int row = quarter * 32 + lane;
-        const uint32_t taddr = tmem + (uint32_t(quarter * 32) << 16) + half * C::kCols;
-        uint32_t it = 0;
+        const uint32_t taddr = tmem + (uint32_t(quarter * 32) << 16) + part * C::kCols;
+        uint32_t it = 0, group = 0;
         bool ok = true;
         BlockWalk<BN, kGrouped> walk(p, tables, first, step);
         BlockTile t;
         while (ok && walk.next(t)) {
-            uint64_t acc[C::kCols / 2];
+            float acc[C::kCols];
 #pragma unroll
-            for (int i = 0; i < C::kCols / 2; ++i) acc[i] = 0;
+            for (int i = 0; i < C::kCols; ++i) acc[i] = 0.0f;
             const bool row_ok = row < t.valid;
             const bool busy = quarter * 32 < t.valid;  // warp-uniform
-            const float* const pa = p.sfa + int64_t(t.row0 + (row_ok ? row : 0)) * p.k_tiles;
-            const int n_block = min((t.n0 + (BN == 256 ? half * C::kCols : 0)) / 128, p.n_blocks - 1);
-            const float* const pb = kRowScales ? nullptr : p.sfb + (int64_t(t.expert) * p.n_blocks + n_block) * p.k_tiles;
-            // the scales of four k-tiles are loaded while the four before them are worked on
-            float na[4], nb[4];
-            const auto load_scales = [&](int k0) {
+            for (int k0 = k_begin; ok && k0 < k_end; k0 += kGroupK, ++group) {
+                const uint32_t slot = group % kScaleSlots;
+                ok = wait_bar<true>(ptx::smem_u32(&bars->sf_full[slot]), (group / kScaleSlots) & 1u, abort, kStatusEpilogue);
+                if (!ok) break;
+                const float* const from = scales + slot * (kGroupK * C::kScales);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    na[i] = nb[i] = 0.0f;
-                    if (k0 + i < k_end) {
-                        na[i] = __ldg(pa + k0 + i);
-                        if (!kRowScales) nb[i] = __ldg(pb + k0 + i);
-                    }
-                }
-            };
-            load_scales(k_begin);
-            for (int k0 = k_begin; ok && k0 < k_end; k0 += 4) {
-                float sc[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sc[i] = kRowScales ? na[i] : na[i] * nb[i];
-                load_scales(k0 + 4);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < kGroupK; ++i) {
                     if (k0 + i >= k_end) break;
-                    const uint32_t buf = it % C::kBufs, slot = it % kScaleSlots;
-                    if constexpr (kRowScales) {
-                        ok = wait_bars<true>(ptx::smem_u32(&bars->acc_full[buf]), (it / C::kBufs) & 1u, true, ptx::smem_u32(&bars->sf_full[slot]),
-                                       (it / kScaleSlots) & 1u, abort, kStatusEpilogue);
-                    } else {
-                        ok = wait_bar<true>(ptx::smem_u32(&bars->acc_full[buf]), (it / C::kBufs) & 1u, abort, kStatusEpilogue);
-                    }
+                    const uint32_t buf = it % C::kBufs;
+                    const float s = from[i * C::kScales + (C::kWeightBlocks == 2 ? part * 2 / kParts * kTileM : 0) + row];
+                    ok = wait_bar<true>(ptx::smem_u32(&bars->acc_full[buf]), (it / C::kBufs) & 1u, abort, kStatusEpilogue);
                     if (!ok) break;
                     if (busy) {
                         ptx::tc_fence_after();
-                        const uint64_t s2 = pack2(__float_as_uint(sc[i]), __float_as_uint(sc[i]));
-                        const float* const col_scales = scales + slot * BN + half * C::kCols;
-                        uint32_t r[2][16];
-                        load_32x16(taddr + buf * BN, r[0]);
+                        const float* const col_scales = from + i * C::kScales + kTileM + part * C::kCols;
+                        constexpr int kLd = C::kLd;
 #pragma unroll
-                        for (int c = 0; c < C::kCols / 16; ++c) {
-                            load_wait(r[c & 1]);
-                            if (c + 1 < C::kCols / 16) load_32x16(taddr + buf * BN + (c + 1) * 16, r[(c + 1) & 1]);
-                            if (c + 1 == C::kCols / 16) {
+                        for (int c = 0; c < C::kCols; c += kLd) {
+                            uint32_t r[kLd];
+                            load_columns(taddr + buf * BN + c, r);
+                            load_wait(r);
+                            if (c + kLd == C::kCols) {
                                 ptx::tc_fence_before();
                                 __syncwarp();
                                 if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&bars->acc_empty[buf]));
                             }
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                uint64_t v = pack2(r[c & 1][2 * j], r[c & 1][2 * j + 1]);
+                            for (int j = 0; j < kLd; j += 4) {
                                 if constexpr (kRowScales) {
-                                    v = mul2(v, *reinterpret_cast<const uint64_t*>(col_scales + c * 16 + 2 * j));
+                                    const float4 w = *reinterpret_cast<const float4*>(col_scales + c + j);
+                                    scale2(r[j], r[j + 1], w.x, w.y);
+                                    scale2(r[j + 2], r[j + 3], w.z, w.w);
                                 }
-                                acc[c * 8 + j] = fma2(v, s2, acc[c * 8 + j]);
+                                add_scaled2(acc[c + j], acc[c + j + 1], r[j], r[j + 1], s);
+                                add_scaled2(acc[c + j + 2], acc[c + j + 3], r[j + 2], r[j + 3], s);
                             }
                         }
                     } else if (lane == 0) {
                         ptx::mbar_arrive(ptx::smem_u32(&bars->acc_empty[buf]));
                     }
-                    if constexpr (kRowScales) {
-                        __syncwarp();
-                        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&bars->sf_empty[slot]));
-                    }
                     ++it;
                 }
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&bars->sf_empty[slot]));
             }
             if (!ok) break;
             if constexpr (kSplit) {
                 // this CTA's sums into its own ring, which nothing uses any more (the last MMAs are done); lines of BN + 4 values
                 // keep the lanes' 16-byte stores apart
                 if (busy) {
-                    float* const line = reinterpret_cast<float*>(smem) + row * (BN + 4) + half * C::kCols;
+                    float* const line = reinterpret_cast<float*>(smem) + row * (BN + 4) + part * C::kCols;
 #pragma unroll
-                    for (int c = 0; c < C::kCols / 4; ++c) {
-                        float4 v;
-                        unpack2(acc[2 * c], v.x, v.y);
-                        unpack2(acc[2 * c + 1], v.z, v.w);
-                        *reinterpret_cast<float4*>(line + c * 4) = v;
+                    for (int c = 0; c < C::kCols; c += 4) {
+                        *reinterpret_cast<float4*>(line + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
                     }
                 }
             } else if (row_ok) {
-                const int col = t.n0 + half * C::kCols;
+                const int col = t.n0 + part * C::kCols;
                 const int64_t at = int64_t(t.row0 + row) * p.ldo + col;
 #pragma unroll
                 for (int c = 0; c < C::kCols / 16; ++c) {
                     if (col + c * 16 >= p.n) break;
                     float f[16];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) unpack2(acc[c * 8 + j], f[2 * j], f[2 * j + 1]);
+                    for (int j = 0; j < 16; ++j) f[j] = acc[c * 16 + j];
                     store_values<16>(f, p.out, at + c * 16, p.n - col - c * 16, p.out_type, p.out_align);
                 }
             }
@@ -561,7 +593,7 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     __syncthreads();
     // no CTA leaves while another reads its sums
     if constexpr (kSplit) ptx::cluster_sync();
-    if (warp == 9) {
+    if (warp == kMmaWarp) {
         ptx::tc_fence_after();
         ptx::tmem_dealloc<1>(tmem, C::kTmemCols);
     }
@@ -691,6 +723,7 @@ int block_gemm(const void* a, const void* b, const float* sfa, const float* sfb,
     p.sfa = sfa, p.sfb = sfb, p.out = out, p.offsets = offsets, p.ldo = ldo;
     p.m = int(m), p.n = int(n), p.k_tiles = int((k + kBlockK - 1) / kBlockK);
     p.n_blocks = int((n + 127) / 128), p.experts = int(experts), p.out_type = out_type, p.pdl = use_pdl != 0;
+    p.wide_scales = aligned(sfa, 16) && aligned(sfb, 16);
     const int64_t row_bytes = ldo * size;
     p.out_align = aligned(out, 32) && row_bytes % 32 == 0 ? 32 : aligned(out, 16) && row_bytes % 16 == 0 ? 16 : size;
     // Rows of `a` per copy: all of a tile's, or about those of a run, so that short runs do not read their neighbours' rows.
