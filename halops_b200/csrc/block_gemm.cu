@@ -62,7 +62,7 @@ struct BlockCfg {
     static constexpr int kScaleBytes = kScaleSlots * kGroupK * kScales * 4;
     static constexpr int kExtra = kBarBytes + kTableBytes + kScaleBytes + 1024;
     static constexpr int kFit = (kSmemBudget - kExtra) / kStageBytes;
-    static constexpr int kStages = kFit > 8 ? 8 : kFit;
+    static constexpr int kStages = kFit > 8 ? 8 : kFit / 2 * 2;
     static constexpr int kSmemBytes = kStages * kStageBytes + kExtra;
     static constexpr int kBufs = BN == 256 ? 2 : 4;
     static constexpr int kTmemCols = kBufs * BN;
@@ -71,6 +71,7 @@ struct BlockCfg {
     static constexpr int kThreads = (kPromoWarps + 4) * 32;
     // BN = 256: 128 accumulators a thread; the third warpgroup gives registers to the other two (168 * 384 = 208 * 256 + 88 * 128)
     static constexpr bool kRegSplit = BN == 256;
+    static_assert(kStages % 2 == 0 && kBufs % 2 == 0, "each stage and buffer belongs to one MMA issuer");
     static_assert(sizeof(BlockBars) <= kBarBytes && kStages >= 3 && kTmemCols <= 512, "budgets");
     static_assert(kTileM * (BN + 4) * 4 <= kStages * kStageBytes, "split-K partial sums fit into the ring");
 };
@@ -363,11 +364,21 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
             const uint32_t bytes = uint32_t(boxes * p.box_rows * kBlockK + C::kBBytes);
             for (int kt = k_begin; kt < k_end; ++kt, ++it) {
                 const uint32_t s = it % C::kStages;
-                ok = wait_bar<true>(ptx::smem_u32(&bars->empty[s]), ((it / C::kStages) & 1u) ^ 1u, abort, kStatusProducer);
+                ok = wait_bar<C::kRegSplit>(ptx::smem_u32(&bars->empty[s]), ((it / C::kStages) & 1u) ^ 1u, abort, kStatusProducer);
                 if (!ok) break;
                 const uint32_t full = ptx::smem_u32(&bars->full[s]);
-                if (ptx::elect_one()) ptx::mbar_arrive_expect_tx(full, bytes);
-                if (ptx::elect_one()) ptx::tma_load_2d(b_base + s * C::kBBytes, &tm_b, kt * kBlockK, b_row, full);
+                if (boxes == 1) {
+                    if (ptx::elect_one()) {
+                        ptx::mbar_arrive_expect_tx(full, bytes);
+                        ptx::tma_load_2d(b_base + s * C::kBBytes, &tm_b, kt * kBlockK, b_row, full);
+                        ptx::tma_load_2d(a_base + s * C::kABytes, &tm_a, kt * kBlockK, t.row0, full);
+                    }
+                    continue;
+                }
+                if (ptx::elect_one()) {
+                    ptx::mbar_arrive_expect_tx(full, bytes);
+                    ptx::tma_load_2d(b_base + s * C::kBBytes, &tm_b, kt * kBlockK, b_row, full);
+                }
                 for (int b = 0; b < boxes; ++b) {
                     if (ptx::elect_one()) {
                         ptx::tma_load_2d(a_base + s * C::kABytes + b * p.box_rows * kBlockK, &tm_a, kt * kBlockK, t.row0 + b * p.box_rows, full);
@@ -376,12 +387,19 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
             }
         }
         ptx::pdl_launch_dependents();
+        // the releases of the last stages arrive in this CTA's shared memory: it is not left before they have
+        for (uint32_t d = it > uint32_t(C::kStages) ? it - C::kStages : 0u; ok && d < it; ++d) {
+            ok = wait_bar<C::kRegSplit>(ptx::smem_u32(&bars->empty[d % C::kStages]), (d / C::kStages) & 1u, abort, kStatusProducer);
+        }
     } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
         // ------------------------------------------------------------ MMA issuers
-        // Every other k-tile each: every k-tile has a buffer of its own, so that nothing has to be kept in order between them.
+        // Every other k-tile each: every k-tile has a buffer of its own, so that nothing has to be kept in order between them.  Stages and
+        // buffers are even in number, so each belongs to one issuer, which waits for all of its phases in turn: one that skipped a
+        // phase would find the wait for the next but one over before it began.
         // float32 sums, e4m3 operands, both K-major; N >> 3, M >> 4
         constexpr uint32_t idesc = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(kTileM >> 4) << 24);
         const uint32_t mine = warp == kMmaWarp ? 0u : 1u;
+        const uint64_t adesc0 = ptx::smem_desc(a_base, 16, 1024, 2), bdesc0 = ptx::smem_desc(b_base, 16, 1024, 2);
         uint32_t it = 0;
         bool ok = true;
         BlockWalk<BN, kGrouped> walk(p, tables, first, step);
@@ -390,20 +408,21 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
             for (int kt = k_begin; kt < k_end; ++kt, ++it) {
                 if ((it & 1u) != mine) continue;
                 const uint32_t s = it % C::kStages, buf = it % C::kBufs;
-                ok = wait_bars<true>(ptx::smem_u32(&bars->full[s]), (it / C::kStages) & 1u, true, ptx::smem_u32(&bars->acc_empty[buf]),
+                ok = wait_bars<C::kRegSplit>(ptx::smem_u32(&bars->full[s]), (it / C::kStages) & 1u, true, ptx::smem_u32(&bars->acc_empty[buf]),
                                ((it / C::kBufs) & 1u) ^ 1u, abort, kStatusMma);
                 if (!ok) break;
                 ptx::tc_fence_after();
-                const uint64_t adesc = ptx::smem_desc(a_base + s * C::kABytes, 16, 1024, 2);
-                const uint64_t bdesc = ptx::smem_desc(b_base + s * C::kBBytes, 16, 1024, 2);
+                // (addresses are in the descriptors' low bits, in units of 16 bytes; K = 32 bytes is a step of 2 inside of the swizzle atom)
+                const uint64_t adesc = adesc0 + s * (C::kABytes >> 4), bdesc = bdesc0 + s * (C::kBBytes >> 4);
                 const uint32_t d = tmem + buf * BN;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    // K = 32 bytes: the start address moves inside of the 128-byte swizzle atom
-                    if (ptx::elect_one()) mma_e4m3(d, adesc + 2 * j, bdesc + 2 * j, idesc, j > 0 ? 1u : 0u);
+                if (ptx::elect_one()) {
+                    mma_e4m3(d, adesc, bdesc, idesc, 0u);
+                    mma_e4m3(d, adesc + 2, bdesc + 2, idesc, 1u);
+                    mma_e4m3(d, adesc + 4, bdesc + 4, idesc, 1u);
+                    mma_e4m3(d, adesc + 6, bdesc + 6, idesc, 1u);
+                    ptx::tc_commit(ptx::smem_u32(&bars->acc_full[buf]));
+                    ptx::tc_commit(ptx::smem_u32(&bars->empty[s]));
                 }
-                if (ptx::elect_one()) ptx::tc_commit(ptx::smem_u32(&bars->acc_full[buf]));
-                if (ptx::elect_one()) ptx::tc_commit(ptx::smem_u32(&bars->empty[s]));
             }
         }
     } else if (warp == kScaleWarp) {
@@ -442,7 +461,7 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
                     }
                 }
                 const uint32_t slot = group % kScaleSlots;
-                ok = wait_bar<true>(ptx::smem_u32(&bars->sf_empty[slot]), ((group / kScaleSlots) & 1u) ^ 1u, abort, kStatusProducer);
+                ok = wait_bar<C::kRegSplit>(ptx::smem_u32(&bars->sf_empty[slot]), ((group / kScaleSlots) & 1u) ^ 1u, abort, kStatusProducer);
                 if (!ok) break;
                 float* const to = scales + slot * (kGroupK * C::kScales) + lane;
 #pragma unroll
@@ -484,7 +503,7 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
             const bool busy = quarter * 32 < t.valid;  // warp-uniform
             for (int k0 = k_begin; ok && k0 < k_end; k0 += kGroupK, ++group) {
                 const uint32_t slot = group % kScaleSlots;
-                ok = wait_bar<true>(ptx::smem_u32(&bars->sf_full[slot]), (group / kScaleSlots) & 1u, abort, kStatusEpilogue);
+                ok = wait_bar<C::kRegSplit>(ptx::smem_u32(&bars->sf_full[slot]), (group / kScaleSlots) & 1u, abort, kStatusEpilogue);
                 if (!ok) break;
                 const float* const from = scales + slot * (kGroupK * C::kScales);
 #pragma unroll
@@ -492,7 +511,7 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
                     if (k0 + i >= k_end) break;
                     const uint32_t buf = it % C::kBufs;
                     const float s = from[i * C::kScales + (C::kWeightBlocks == 2 ? part * 2 / kParts * kTileM : 0) + row];
-                    ok = wait_bar<true>(ptx::smem_u32(&bars->acc_full[buf]), (it / C::kBufs) & 1u, abort, kStatusEpilogue);
+                    ok = wait_bar<C::kRegSplit>(ptx::smem_u32(&bars->acc_full[buf]), (it / C::kBufs) & 1u, abort, kStatusEpilogue);
                     if (!ok) break;
                     if (busy) {
                         ptx::tc_fence_after();
