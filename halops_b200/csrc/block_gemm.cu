@@ -41,8 +41,8 @@ constexpr int kScaleSlots = 2;  // such groups in shared memory
 struct BlockBars {
     uint64_t full[8];
     uint64_t empty[8];
-    uint64_t acc_full[4];
-    uint64_t acc_empty[4];
+    uint64_t acc_full[2];
+    uint64_t acc_empty[2];
     uint64_t sf_full[kScaleSlots];
     uint64_t sf_empty[kScaleSlots];
     uint32_t tmem_base;
@@ -51,9 +51,12 @@ struct BlockBars {
 
 template <int BN, bool kRowScales>
 struct BlockCfg {
-    static constexpr int kABytes = kTileM * kBlockK;
+    // k-tiles of a step, which share a stage and a set of buffers: what a step's waits and signals cost (400 to 500 cycles from role to
+    // role) is more than a narrow tile's k-tile has to do, 8192 columns of 64 x 16 rows x 7168 take XX us with steps of two and XX of one
+    static constexpr int kStep = BN == 256 ? 1 : 2;
+    static constexpr int kABytes = kTileM * kBlockK;  // per k-tile
     static constexpr int kBBytes = BN * kBlockK;
-    static constexpr int kStageBytes = kABytes + kBBytes;
+    static constexpr int kStageBytes = kStep * (kABytes + kBBytes);
     static constexpr int kBarBytes = 512;
     static constexpr int kTableBytes = (kMaxExperts + 8) * 8;                // grouped: row tiles before, first row of, each expert
     static constexpr int kWeightBlocks = kRowScales ? 1 : (BN + 127) / 128;  // blocks of 128 weight rows that a tile spans
@@ -62,17 +65,17 @@ struct BlockCfg {
     static constexpr int kScaleBytes = kScaleSlots * kGroupK * kScales * 4;
     static constexpr int kExtra = kBarBytes + kTableBytes + kScaleBytes + 1024;
     static constexpr int kFit = (kSmemBudget - kExtra) / kStageBytes;
-    static constexpr int kStages = kFit > 8 ? 8 : kFit / 2 * 2;
+    static constexpr int kStages = kStep == 1 ? kFit / 2 * 2 : kFit;
     static constexpr int kSmemBytes = kStages * kStageBytes + kExtra;
-    static constexpr int kBufs = BN == 256 ? 2 : 4;
-    static constexpr int kTmemCols = kBufs * BN;
+    static constexpr int kBufs = 2;  // of kStep accumulators each
+    static constexpr int kTmemCols = kBufs * kStep * BN;
     static constexpr int kCols = BN / kParts;  // columns of a promotion warp
-    static constexpr int kLd = BN == 256 ? 16 : kCols < 32 ? kCols : 32;  // of which one load brings
+    static constexpr int kLd = BN == 64 ? 32 : 16;  // of which one load brings
     static constexpr int kThreads = (kPromoWarps + 4) * 32;
     // BN = 256: 128 accumulators a thread; the third warpgroup gives registers to the other two (168 * 384 = 208 * 256 + 88 * 128)
     static constexpr bool kRegSplit = BN == 256;
-    static_assert(kStages % 2 == 0 && kBufs % 2 == 0, "each stage and buffer belongs to one MMA issuer");
-    static_assert(sizeof(BlockBars) <= kBarBytes && kStages >= 3 && kTmemCols <= 512, "budgets");
+    static_assert(kStep == 2 || (kStages % 2 == 0 && kBufs % 2 == 0), "each stage and buffer belongs to one MMA issuer");
+    static_assert(sizeof(BlockBars) <= kBarBytes && kStages >= 3 && kStages <= 8 && kTmemCols <= 512, "budgets");
     static_assert(kTileM * (BN + 4) * 4 <= kStages * kStageBytes, "split-K partial sums fit into the ring");
 };
 
@@ -273,7 +276,7 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     extern __shared__ __align__(16) uint8_t smem_raw[];
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t a_base = ptx::smem_u32(smem);
-    const uint32_t b_base = a_base + C::kStages * C::kABytes;
+    const uint32_t b_base = a_base + C::kStages * C::kStep * C::kABytes;
     constexpr int kBarOffset = C::kStages * C::kStageBytes;
     BlockBars* const bars = reinterpret_cast<BlockBars*>(smem + kBarOffset);
     int* const tables = reinterpret_cast<int*>(smem + kBarOffset + C::kBarBytes);
@@ -285,10 +288,10 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::kStages; ++s) {
             ptx::mbar_init(ptx::smem_u32(&bars->full[s]), 1);
-            ptx::mbar_init(ptx::smem_u32(&bars->empty[s]), 1);
+            ptx::mbar_init(ptx::smem_u32(&bars->empty[s]), C::kStep);  // one commit per k-tile
         }
         for (int s = 0; s < C::kBufs; ++s) {
-            ptx::mbar_init(ptx::smem_u32(&bars->acc_full[s]), 1);
+            ptx::mbar_init(ptx::smem_u32(&bars->acc_full[s]), C::kStep);
             ptx::mbar_init(ptx::smem_u32(&bars->acc_empty[s]), kPromoWarps);
         }
         for (int s = 0; s < kScaleSlots; ++s) {
@@ -347,8 +350,10 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     const int rank = kSplit ? int(blockIdx.x) % p.split : 0;
     const int first = kSplit ? int(blockIdx.x) / p.split : int(blockIdx.x);
     const int step = kSplit ? int(gridDim.x) / p.split : int(gridDim.x);
-    const int k_begin = kSplit ? int(int64_t(p.k_tiles) * rank / p.split) : 0;
-    const int k_end = kSplit ? int(int64_t(p.k_tiles) * (rank + 1) / p.split) : p.k_tiles;
+    // (whole steps per CTA of a cluster; a step that sticks out beyond K reads zeros there and has zeros for scales)
+    const int steps = (p.k_tiles + C::kStep - 1) / C::kStep;
+    const int k_begin = kSplit ? int(int64_t(steps) * rank / p.split) * C::kStep : 0;
+    const int k_end = kSplit ? min(int(int64_t(steps) * (rank + 1) / p.split) * C::kStep, p.k_tiles) : p.k_tiles;
 
     if (warp >= kPromoWarps) {
     if constexpr (C::kRegSplit) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
@@ -361,27 +366,28 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         while (ok && walk.next(t)) {
             const int boxes = (t.valid + p.box_rows - 1) / p.box_rows;
             const int b_row = t.expert * p.n + t.n0;
-            const uint32_t bytes = uint32_t(boxes * p.box_rows * kBlockK + C::kBBytes);
-            for (int kt = k_begin; kt < k_end; ++kt, ++it) {
+            const uint32_t bytes = C::kStep * uint32_t(boxes * p.box_rows * kBlockK + C::kBBytes);
+            for (int kt = k_begin; kt < k_end; kt += C::kStep, ++it) {
                 const uint32_t s = it % C::kStages;
                 ok = wait_bar<C::kRegSplit>(ptx::smem_u32(&bars->empty[s]), ((it / C::kStages) & 1u) ^ 1u, abort, kStatusProducer);
                 if (!ok) break;
                 const uint32_t full = ptx::smem_u32(&bars->full[s]);
-                if (boxes == 1) {
-                    if (ptx::elect_one()) {
-                        ptx::mbar_arrive_expect_tx(full, bytes);
-                        ptx::tma_load_2d(b_base + s * C::kBBytes, &tm_b, kt * kBlockK, b_row, full);
-                        ptx::tma_load_2d(a_base + s * C::kABytes, &tm_a, kt * kBlockK, t.row0, full);
-                    }
-                    continue;
-                }
+                const uint32_t a_to = a_base + s * (C::kStep * C::kABytes), b_to = b_base + s * (C::kStep * C::kBBytes);
                 if (ptx::elect_one()) {
                     ptx::mbar_arrive_expect_tx(full, bytes);
-                    ptx::tma_load_2d(b_base + s * C::kBBytes, &tm_b, kt * kBlockK, b_row, full);
+#pragma unroll
+                    for (int u = 0; u < C::kStep; ++u) {
+                        ptx::tma_load_2d(b_to + u * C::kBBytes, &tm_b, (kt + u) * kBlockK, b_row, full);
+                        ptx::tma_load_2d(a_to + u * C::kABytes, &tm_a, (kt + u) * kBlockK, t.row0, full);
+                    }
                 }
-                for (int b = 0; b < boxes; ++b) {
+                for (int b = 1; b < boxes; ++b) {
+                    const int skip = b * p.box_rows;
                     if (ptx::elect_one()) {
-                        ptx::tma_load_2d(a_base + s * C::kABytes + b * p.box_rows * kBlockK, &tm_a, kt * kBlockK, t.row0 + b * p.box_rows, full);
+#pragma unroll
+                        for (int u = 0; u < C::kStep; ++u) {
+                            ptx::tma_load_2d(a_to + u * C::kABytes + skip * kBlockK, &tm_a, (kt + u) * kBlockK, t.row0 + skip, full);
+                        }
                     }
                 }
             }
@@ -393,9 +399,9 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         }
     } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
         // ------------------------------------------------------------ MMA issuers
-        // Every other k-tile each: every k-tile has a buffer of its own, so that nothing has to be kept in order between them.  Stages and
-        // buffers are even in number, so each belongs to one issuer, which waits for all of its phases in turn: one that skipped a
-        // phase would find the wait for the next but one over before it began.
+        // Every k-tile has a buffer of its own, so nothing has to be kept in order between the two.  Steps of two: a k-tile of every step each.
+        // Steps of one: every other step each; stages and buffers are then even in number, so that each belongs to one issuer, which waits
+        // for all of its phases in turn (one that skipped a phase would find the wait for the next but one over before it began).
         // float32 sums, e4m3 operands, both K-major; N >> 3, M >> 4
         constexpr uint32_t idesc = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(kTileM >> 4) << 24);
         const uint32_t mine = warp == kMmaWarp ? 0u : 1u;
@@ -405,16 +411,16 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         BlockWalk<BN, kGrouped> walk(p, tables, first, step);
         BlockTile t;
         while (ok && walk.next(t)) {
-            for (int kt = k_begin; kt < k_end; ++kt, ++it) {
-                if ((it & 1u) != mine) continue;
-                const uint32_t s = it % C::kStages, buf = it % C::kBufs;
+            for (int kt = k_begin; kt < k_end; kt += C::kStep, ++it) {
+                if (C::kStep == 1 && (it & 1u) != mine) continue;
+                const uint32_t s = it % C::kStages, buf = it % C::kBufs, u = C::kStep == 1 ? 0u : mine;
                 ok = wait_bars<C::kRegSplit>(ptx::smem_u32(&bars->full[s]), (it / C::kStages) & 1u, true, ptx::smem_u32(&bars->acc_empty[buf]),
                                ((it / C::kBufs) & 1u) ^ 1u, abort, kStatusMma);
                 if (!ok) break;
                 ptx::tc_fence_after();
                 // (addresses are in the descriptors' low bits, in units of 16 bytes; K = 32 bytes is a step of 2 inside of the swizzle atom)
-                const uint64_t adesc = adesc0 + s * (C::kABytes >> 4), bdesc = bdesc0 + s * (C::kBBytes >> 4);
-                const uint32_t d = tmem + buf * BN;
+                const uint64_t adesc = adesc0 + (s * C::kStep + u) * (C::kABytes >> 4), bdesc = bdesc0 + (s * C::kStep + u) * (C::kBBytes >> 4);
+                const uint32_t d = tmem + (buf * C::kStep + u) * BN;
                 if (ptx::elect_one()) {
                     mma_e4m3(d, adesc, bdesc, idesc, 0u);
                     mma_e4m3(d, adesc + 2, bdesc + 2, idesc, 1u);
@@ -507,35 +513,41 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
                 if (!ok) break;
                 const float* const from = scales + slot * (kGroupK * C::kScales);
 #pragma unroll
-                for (int i = 0; i < kGroupK; ++i) {
+                for (int i = 0; i < kGroupK; i += C::kStep) {
                     if (k0 + i >= k_end) break;
                     const uint32_t buf = it % C::kBufs;
-                    const float s = from[i * C::kScales + (C::kWeightBlocks == 2 ? part * 2 / kParts * kTileM : 0) + row];
+                    float s[C::kStep];
+#pragma unroll
+                    for (int u = 0; u < C::kStep; ++u) s[u] = from[(i + u) * C::kScales + (C::kWeightBlocks == 2 ? part * 2 / kParts * kTileM : 0) + row];
                     ok = wait_bar<C::kRegSplit>(ptx::smem_u32(&bars->acc_full[buf]), (it / C::kBufs) & 1u, abort, kStatusEpilogue);
                     if (!ok) break;
                     if (busy) {
                         ptx::tc_fence_after();
-                        const float* const col_scales = from + i * C::kScales + kTileM + part * C::kCols;
                         constexpr int kLd = C::kLd;
 #pragma unroll
                         for (int c = 0; c < C::kCols; c += kLd) {
-                            uint32_t r[kLd];
-                            load_columns(taddr + buf * BN + c, r);
-                            load_wait(r);
+                            uint32_t r[C::kStep][kLd];
+#pragma unroll
+                            for (int u = 0; u < C::kStep; ++u) load_columns(taddr + (buf * C::kStep + u) * BN + c, r[u]);
+#pragma unroll
+                            for (int u = 0; u < C::kStep; ++u) load_wait(r[u]);
                             if (c + kLd == C::kCols) {
                                 ptx::tc_fence_before();
                                 __syncwarp();
                                 if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&bars->acc_empty[buf]));
                             }
 #pragma unroll
-                            for (int j = 0; j < kLd; j += 4) {
-                                if constexpr (kRowScales) {
-                                    const float4 w = *reinterpret_cast<const float4*>(col_scales + c + j);
-                                    scale2(r[j], r[j + 1], w.x, w.y);
-                                    scale2(r[j + 2], r[j + 3], w.z, w.w);
+                            for (int u = 0; u < C::kStep; ++u) {
+#pragma unroll
+                                for (int j = 0; j < kLd; j += 4) {
+                                    if constexpr (kRowScales) {
+                                        const float4 w = *reinterpret_cast<const float4*>(from + (i + u) * C::kScales + kTileM + part * C::kCols + c + j);
+                                        scale2(r[u][j], r[u][j + 1], w.x, w.y);
+                                        scale2(r[u][j + 2], r[u][j + 3], w.z, w.w);
+                                    }
+                                    add_scaled2(acc[c + j], acc[c + j + 1], r[u][j], r[u][j + 1], s[u]);
+                                    add_scaled2(acc[c + j + 2], acc[c + j + 3], r[u][j + 2], r[u][j + 3], s[u]);
                                 }
-                                add_scaled2(acc[c + j], acc[c + j + 1], r[j], r[j + 1], s);
-                                add_scaled2(acc[c + j + 2], acc[c + j + 3], r[j + 2], r[j + 3], s);
                             }
                         }
                     } else if (lane == 0) {
