@@ -185,6 +185,16 @@ __device__ __forceinline__ void load_wait(uint32_t (&r)[16]) {
                  : "memory");
 }
 
+// 16 lanes x 32 columns as fragments of 8 x 8: register 4 g + 2 h + i is row lane / 4 + 8 h, column 8 g + 2 (lane % 4) + i.
+__device__ __forceinline__ void load_fragments(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+
 // (a, b) += (x, y) * s as one packed instruction.  It needs the issue slots of two scalar ones, but not their operand reads: 128 columns
 // of 8 warps, loads included, take 292 cycles with it and 421 with fmaf.
 __device__ __forceinline__ void add_scaled2(float& a, float& b, uint32_t x, uint32_t y, float s) {
@@ -241,8 +251,18 @@ __device__ __forceinline__ void store_values(const float (&f)[kN], void* out, in
     if (type == HQ_DTYPE_FP32) {
         float* const o = static_cast<float*>(out) + at;
         if (left >= kN && align >= 16) {
+            if constexpr (kN >= 8) {
 #pragma unroll
-            for (int i = 0; i < kN; i += 4) *reinterpret_cast<float4*>(o + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+                for (int i = 0; i < kN; i += 8) {
+                    uint32_t w[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(f[i + j]);
+                    store_32_bytes(o + i, w, align);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < kN; i += 2) *reinterpret_cast<float2*>(o + i) = make_float2(f[i], f[i + 1]);
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < kN; ++i) {
@@ -258,8 +278,10 @@ __device__ __forceinline__ void store_values(const float (&f)[kN], void* out, in
     if (left >= kN && align >= 16) {
         if constexpr (kN == 16) {
             store_32_bytes(o, w, align);
-        } else {
+        } else if constexpr (kN == 4) {
             *reinterpret_cast<uint2*>(o) = make_uint2(w[0], w[1]);
+        } else {
+            *reinterpret_cast<uint32_t*>(o) = w[0];
         }
     } else {
 #pragma unroll
@@ -516,37 +538,68 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
                 for (int i = 0; i < kGroupK; i += C::kStep) {
                     if (k0 + i >= k_end) break;
                     const uint32_t buf = it % C::kBufs;
-                    float s[C::kStep];
+                    float s[C::kStep][kRowScales ? 4 : 1];
 #pragma unroll
-                    for (int u = 0; u < C::kStep; ++u) s[u] = from[(i + u) * C::kScales + (C::kWeightBlocks == 2 ? part * 2 / kParts * kTileM : 0) + row];
+                    for (int u = 0; u < C::kStep; ++u) {
+                        if constexpr (kRowScales) {
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) s[u][q] = from[(i + u) * C::kScales + quarter * 32 + q * 8 + lane / 4];
+                        } else {
+                            s[u][0] = from[(i + u) * C::kScales + (C::kWeightBlocks == 2 ? part * 2 / kParts * kTileM : 0) + row];
+                        }
+                    }
                     ok = wait_bar<C::kRegSplit>(ptx::smem_u32(&bars->acc_full[buf]), (it / C::kBufs) & 1u, abort, kStatusEpilogue);
                     if (!ok) break;
                     if (busy) {
                         ptx::tc_fence_after();
-                        constexpr int kLd = C::kLd;
+                        const auto drained = [&] {
+                            ptx::tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&bars->acc_empty[buf]));
+                        };
+                        if constexpr (kRowScales) {
+                            // fragments: a thread has 4 rows and 2 of 8 columns, so that it reads a quarter of the columns' scales (with a row and
+                            // all columns, the shared-memory reads of 128 x 128 scales a k-tile took longer than its products)
 #pragma unroll
-                        for (int c = 0; c < C::kCols; c += kLd) {
-                            uint32_t r[C::kStep][kLd];
+                            for (int c = 0; c < C::kCols; c += 32) {
 #pragma unroll
-                            for (int u = 0; u < C::kStep; ++u) load_columns(taddr + (buf * C::kStep + u) * BN + c, r[u]);
+                                for (int u = 0; u < C::kStep; ++u) {
+                                    uint32_t r[2][16];
+                                    load_fragments(taddr + (buf * C::kStep + u) * BN + c, r[0]);
+                                    load_fragments(taddr + (16u << 16) + (buf * C::kStep + u) * BN + c, r[1]);
+                                    const float* const col = from + (i + u) * C::kScales + kTileM + part * C::kCols + c + lane % 4 * 2;
+                                    float2 w[4];
 #pragma unroll
-                            for (int u = 0; u < C::kStep; ++u) load_wait(r[u]);
-                            if (c + kLd == C::kCols) {
-                                ptx::tc_fence_before();
-                                __syncwarp();
-                                if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&bars->acc_empty[buf]));
-                            }
+                                    for (int g = 0; g < 4; ++g) w[g] = *reinterpret_cast<const float2*>(col + g * 8);
+                                    load_wait(r[0]);
+                                    load_wait(r[1]);
+                                    if (c + 32 == C::kCols && u + 1 == C::kStep) drained();
 #pragma unroll
-                            for (int u = 0; u < C::kStep; ++u) {
+                                    for (int g = 0; g < 4; ++g) {
 #pragma unroll
-                                for (int j = 0; j < kLd; j += 4) {
-                                    if constexpr (kRowScales) {
-                                        const float4 w = *reinterpret_cast<const float4*>(from + (i + u) * C::kScales + kTileM + part * C::kCols + c + j);
-                                        scale2(r[u][j], r[u][j + 1], w.x, w.y);
-                                        scale2(r[u][j + 2], r[u][j + 3], w.z, w.w);
+                                        for (int q = 0; q < 4; ++q) {
+                                            uint32_t &x = r[q / 2][g * 4 + q % 2 * 2], &y = r[q / 2][g * 4 + q % 2 * 2 + 1];
+                                            float* const to = acc + c + (g * 4 + q) * 2;
+                                            scale2(x, y, w[g].x, w[g].y);
+                                            add_scaled2(to[0], to[1], x, y, s[u][q]);
+                                        }
                                     }
-                                    add_scaled2(acc[c + j], acc[c + j + 1], r[u][j], r[u][j + 1], s[u]);
-                                    add_scaled2(acc[c + j + 2], acc[c + j + 3], r[u][j + 2], r[u][j + 3], s[u]);
+                                }
+                            }
+                        } else {
+                            constexpr int kLd = C::kLd;
+#pragma unroll
+                            for (int c = 0; c < C::kCols; c += kLd) {
+                                uint32_t r[C::kStep][kLd];
+#pragma unroll
+                                for (int u = 0; u < C::kStep; ++u) load_columns(taddr + (buf * C::kStep + u) * BN + c, r[u]);
+#pragma unroll
+                                for (int u = 0; u < C::kStep; ++u) load_wait(r[u]);
+                                if (c + kLd == C::kCols) drained();
+#pragma unroll
+                                for (int u = 0; u < C::kStep; ++u) {
+#pragma unroll
+                                    for (int j = 0; j < kLd; j += 2) add_scaled2(acc[c + j], acc[c + j + 1], r[u][j], r[u][j + 1], s[u][0]);
                                 }
                             }
                         }
@@ -567,6 +620,20 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
 #pragma unroll
                     for (int c = 0; c < C::kCols; c += 4) {
                         *reinterpret_cast<float4*>(line + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+                    }
+                }
+            } else if constexpr (kRowScales) {
+#pragma unroll
+                for (int c = 0; c < C::kCols; c += 8) {
+                    const int col = t.n0 + part * C::kCols + c + lane % 4 * 2;
+                    if (col >= p.n) continue;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int r = quarter * 32 + q * 8 + lane / 4;
+                        if (r < t.valid) {
+                            const float f[2] = {acc[(c / 8 * 4 + q) * 2], acc[(c / 8 * 4 + q) * 2 + 1]};
+                            store_values<2>(f, p.out, int64_t(t.row0 + r) * p.ldo + col, p.n - col, p.out_type, p.out_align);
+                        }
                     }
                 }
             } else if (row_ok) {
