@@ -52,7 +52,8 @@ struct BlockBars {
 template <int BN, bool kRowScales>
 struct BlockCfg {
     // k-tiles of a step, which share a stage and a set of buffers: what a step's waits and signals cost (400 to 500 cycles from role to
-    // role) is more than a narrow tile's k-tile has to do, 8192 columns of 64 x 16 rows x 7168 take XX us with steps of two and XX of one
+    // role) is more than a narrow tile's k-tile has to do, 16 x 4096 x 7168 on 64 columns takes 11.8 us in steps of two and 13.1 of one,
+    // 8192 x 8192 x 8192 on 128 columns 579 and 615
     static constexpr int kStep = BN == 256 ? 1 : 2;
     static constexpr int kABytes = kTileM * kBlockK;  // per k-tile
     static constexpr int kBBytes = BN * kBlockK;
@@ -740,28 +741,37 @@ struct BlockChoice {
     int bn, split;
 };
 
+// The least time by figures of the three tiles, GEMM alone.  A k-tile takes `alone` microseconds with few CTAs running and `full` with all
+// (then the CTAs share L2 and power): 16 x 4096 x 7168 on 64 columns 11.8 us, 128 x 4096 x 16384 24.9, 8192 x 8192 x 8192 786 (128
+// columns: 14.6, 28.6, 579; 256: -, -, 484 to 558); `tile` is what a tile's end costs, and a launch is 3.  With a CTA's share of
+// K in `split` CTAs of a cluster: 2.2 more for its barriers and the exchange (16 x 4096 x 7168 on 128 columns 15.4 us whole, 9.3
+// in four; 8 x 1024 x 4096 11.2 whole, 6.1 in eight; 1 x 7168 x 2048 6.7 whole, 7.3 in two).
 BlockChoice choose(const BlockProblem& g) {
-    const int k_tiles = g.args.k_tiles;
-    // microseconds of a k-tile and of a tile's end
     struct Cost {
         int bn;
-        double step, tile;
+        double alone, full, tile;
     };
-    constexpr Cost kCosts[] = {{256, 0.36, 2.0}, {128, 0.22, 1.5}, {64, 0.15, 1.2}};
-    BlockChoice best = {64, 1};
+    constexpr Cost kCosts[] = {{128, 0.20, 0.30, 1.0}, {64, 0.157, 0.21, 0.7}, {256, 0.42, 0.53, 1.6}};  // (in order of preference where the floor decides)
+    const int k_tiles = g.args.k_tiles;
+    const int64_t runs = std::min(g.experts, g.rows_a);  // with rows
+    const int64_t mean = (g.rows_a + runs - 1) / runs;
+    const int64_t row_tiles = runs * ((mean + kTileM - 1) / kTileM);  // (of runs of the same length)
+    // the operands and the result pass HBM once at best
+    const double floor_us = (double(g.rows_a) * g.k + double(runs) * g.n * g.k + 2.0 * g.rows_a * g.n) / 6.0e6 + 4.0;
+    BlockChoice best = {128, 1};
     double least = 1e30;
     for (const Cost& c : kCosts) {
         if (g.row_scales && c.bn == 256) continue;
-        int64_t row_tiles = (g.rows_a + kTileM - 1) / kTileM;
-        if (g.grouped) row_tiles = g.rows_a / kTileM + std::min<int64_t>(g.experts, g.rows_a);
         const int64_t tiles = row_tiles * ((g.n + c.bn - 1) / c.bn);
-        int split = 1;
-        if (!g.grouped && !g.row_scales && c.bn <= 128) {
-            while (split < 8 && 2 * split * tiles <= g.sms && k_tiles >= 4 * split) split *= 2;
+        for (int split = 1; split <= 8; split *= 2) {
+            // (clusters of 8 do not fill every group of SMs)
+            if (split > 1 && (g.grouped || g.row_scales || c.bn == 256 || tiles * split > (split == 8 ? g.sms * 6 / 7 : g.sms) || k_tiles < 4 * split)) break;
+            const int64_t ctas = tiles * split, waves = (ctas + g.sms - 1) / g.sms;
+            const double busy = double(std::min<int64_t>(ctas, g.sms)) / g.sms;
+            const double step = c.alone + (c.full - c.alone) * busy;
+            const double t = std::max(floor_us, 3.0 + (split > 1 ? 2.2 : 0.0) + double(waves) * (step * ((k_tiles + split - 1) / split) + c.tile));
+            if (t < least) least = t, best = {c.bn, split};
         }
-        const double waves = double((tiles * split + g.sms - 1) / g.sms);
-        const double t = waves * (c.step * ((k_tiles + split - 1) / split) + c.tile) + (split > 1 ? 2.0 : 0.0);
-        if (t < least) least = t, best = {c.bn, split};
     }
     return best;
 }

@@ -15,6 +15,7 @@
 #include <Python.h>
 
 #include <ATen/PythonTorchFunctionTLS.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -271,6 +272,46 @@ bool given(PyObject* o, c10::IntArrayRef shape, at::ScalarType type, const at::T
     return true;
 }
 
+// A new tensor without the dispatcher: at::empty takes the host 1.2 us, and a small call makes up to four.
+at::Tensor fresh(c10::IntArrayRef shape, at::ScalarType type, c10::Device device) {
+    return at::Tensor(at::detail::empty_cuda(shape, type, device, c10::nullopt));
+}
+
+// Several tensors of one allocation (256-byte aligned), which lives as long as the last of them.
+class Together {
+    int64_t bytes_ = 0;
+    struct Part {
+        at::Tensor* to;
+        c10::IntArrayRef shape;
+        at::ScalarType type;
+        int64_t at;
+    } parts_[4];
+    int n_ = 0;
+
+public:
+    void add(at::Tensor* to, c10::IntArrayRef shape, at::ScalarType type) {
+        int64_t size = int64_t(c10::elementSize(type));
+        for (const int64_t d : shape) size *= d;
+        parts_[n_++] = {to, shape, type, bytes_};
+        bytes_ += (size + 255) / 256 * 256;
+    }
+    void make(c10::Device device) {
+        if (n_ == 0) return;
+        if (n_ == 1) {
+            *parts_[0].to = fresh(parts_[0].shape, parts_[0].type, device);
+            return;
+        }
+        const at::Tensor whole = fresh({bytes_}, at::kByte, device);
+        for (int i = 0; i < n_; ++i) {
+            const Part& p = parts_[i];
+            at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), c10::scalarTypeToTypeMeta(p.type));
+            t.unsafeGetTensorImpl()->set_sizes_contiguous(p.shape);
+            t.unsafeGetTensorImpl()->set_storage_offset(p.at / int64_t(c10::elementSize(p.type)));
+            *p.to = std::move(t);
+        }
+    }
+};
+
 PyObject* pair_or_given(PyObject* a, const at::Tensor& x, PyObject* b, const at::Tensor& y) {
     PyObject* const p = a != Py_None ? Py_NewRef(a) : THPVariable_Wrap(x);
     PyObject* const q = p == nullptr ? nullptr : b != Py_None ? Py_NewRef(b) : THPVariable_Wrap(y);
@@ -304,10 +345,12 @@ PyObject* block_quant(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     const int64_t ld = x->stride(-2), batch = x->dim() == 3 ? x->stride(0) : 0;
     const int dev = x->get_device();
     void* const st = stream_of(*x);
-    const auto on_device = at::TensorOptions().device(x->device());
+    const c10::Device device = x->device();
     if (unlocked([&](char* err) {
-            if (!q.defined()) q = at::empty(qs, on_device.dtype(at::kFloat8_e4m3fn));
-            if (!sf.defined()) sf = at::empty(ss, on_device.dtype(at::kFloat));
+            Together outputs;
+            if (!q.defined()) outputs.add(&q, qs, at::kFloat8_e4m3fn);
+            if (!sf.defined()) outputs.add(&sf, ss, at::kFloat);
+            outputs.make(device);
             return g_fn.block_quant(px, ld, batch, type, e, m, k, rows, transpose, pdl, q.data_ptr(), sf.data_ptr(), dev, st, err, kErrLen);
         }) != 0) {
         Py_RETURN_NONE;
@@ -341,10 +384,12 @@ PyObject* swiglu_block_quant(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     const int64_t ld = x->stride(0);
     const int dev = x->get_device();
     void* const st = stream_of(*x);
-    const auto on_device = at::TensorOptions().device(x->device());
+    const c10::Device device = x->device();
     if (unlocked([&](char* err) {
-            if (!q.defined()) q = at::empty(qs, on_device.dtype(at::kFloat8_e4m3fn));
-            if (!sf.defined()) sf = at::empty(ss, on_device.dtype(at::kFloat));
+            Together outputs;
+            if (!q.defined()) outputs.add(&q, qs, at::kFloat8_e4m3fn);
+            if (!sf.defined()) outputs.add(&sf, ss, at::kFloat);
+            outputs.make(device);
             return g_fn.swiglu(px, ld, type, m, k, limit, pdl, q.data_ptr(), sf.data_ptr(), dev, st, err, kErrLen);
         }) != 0) {
         Py_RETURN_NONE;
@@ -422,13 +467,16 @@ PyObject* moe_sort(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     const void* const p = ids->data_ptr();
     const int dev = ids->get_device();
     void* const st = stream_of(*ids);
-    const auto options = at::TensorOptions().device(ids->device()).dtype(at::kInt);
+    const c10::Device device = ids->device();
+    const int64_t rows_shape[1] = {n_rows}, offsets_shape[1] = {experts + 1};
     at::Tensor out[4];
     if (unlocked([&](char* err) {
-            out[0] = at::empty(ids->sizes(), options);
-            out[1] = at::empty({n_rows}, options);
-            out[2] = at::empty({experts + 1}, options);
-            out[3] = at::empty({n_rows}, options);
+            Together outputs;
+            outputs.add(&out[0], ids->sizes(), at::kInt);
+            outputs.add(&out[1], rows_shape, at::kInt);
+            outputs.add(&out[2], offsets_shape, at::kInt);
+            outputs.add(&out[3], rows_shape, at::kInt);
+            outputs.make(device);
             int32_t* at[4];
             for (int i = 0; i < 4; ++i) at[i] = static_cast<int32_t*>(out[i].data_ptr());
             return g_fn.moe_sort(p, int(ids->element_size()), ids->size(0), ids->size(1), experts, align, n_rows, pdl, at[0], at[1], at[2], at[3],
@@ -494,7 +542,7 @@ PyObject* moe_permute(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     const int dev = x->get_device();
     void* const st = stream_of(*x);
     if (unlocked([&](char* err) {
-            if (!out.defined()) out = at::empty(shape, x->options());
+            if (!out.defined()) out = fresh(shape, x->scalar_type(), x->device());
             return g_fn.moe_permute(px, ld, order.tokens, h * size, order.topk, order.rows, order.pairs, order.offsets, order.experts, order.n_rows,
                                     order.padded, pdl, out.data_ptr(), dev, st, err, kErrLen);
         }) != 0) {
@@ -522,10 +570,12 @@ PyObject* moe_permute_block_quant(PyObject*, PyObject* const* a, Py_ssize_t narg
     const int64_t ld = x->stride(0);
     const int dev = x->get_device();
     void* const st = stream_of(*x);
-    const auto on_device = at::TensorOptions().device(x->device());
+    const c10::Device device = x->device();
     if (unlocked([&](char* err) {
-            if (!q.defined()) q = at::empty(qs, on_device.dtype(at::kFloat8_e4m3fn));
-            if (!sf.defined()) sf = at::empty(ss, on_device.dtype(at::kFloat));
+            Together outputs;
+            if (!q.defined()) outputs.add(&q, qs, at::kFloat8_e4m3fn);
+            if (!sf.defined()) outputs.add(&sf, ss, at::kFloat);
+            outputs.make(device);
             return g_fn.moe_permute_quant(px, ld, type, order.tokens, h, order.topk, order.rows, order.pairs, order.offsets, order.experts,
                                           order.n_rows, order.padded, pdl, q.data_ptr(), sf.data_ptr(), dev, st, err, kErrLen);
         }) != 0) {
@@ -569,7 +619,7 @@ PyObject* moe_unpermute(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     void* const st = stream_of(*z);
     at::Tensor out;
     if (unlocked([&](char* err) {
-            out = at::empty({order.tokens, h}, z->options());
+            out = fresh({order.tokens, h}, z->scalar_type(), z->device());
             return g_fn.moe_unpermute(pz, ld, type, order.n_rows, h, order.tokens, order.topk, order.rows, weights, pdl, out.data_ptr(), dev, st, err,
                                       kErrLen);
         }) != 0) {
@@ -607,8 +657,8 @@ PyObject* moe_unpermute_backward(PyObject*, PyObject* const* a, Py_ssize_t nargs
     const int dev = z->get_device();
     void* const st = stream_of(*z);
     if (unlocked([&](char* err) {
-            if (!gz.defined()) gz = at::empty(shape, z->options());
-            if (a[3] != Py_None) gw = at::empty({order.tokens, order.topk}, z->options().dtype(at::kFloat));
+            if (!gz.defined()) gz = fresh(shape, z->scalar_type(), z->device());
+            if (a[3] != Py_None) gw = fresh({order.tokens, order.topk}, at::kFloat, z->device());
             return g_fn.moe_unpermute_backward(pg, ld_g, pz, ld_z, type, order.n_rows, h, order.tokens, order.topk, order.rows, order.pairs,
                                                order.offsets, order.experts, order.padded, weights, pdl, gz.data_ptr(),
                                                gw.defined() ? static_cast<float*>(gw.data_ptr()) : nullptr, dev, st, err, kErrLen);

@@ -57,11 +57,13 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const Id* __rest
     grid_wait();
     grid_launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x;
-    for (int i = tid; i < kSortWarps * experts; i += kSortThreads) lines[i] = 0;
+    // warps with pairs: few pairs make few lines to zero and to sum over
+    const int used = min(kSortWarps, max(1, (pairs_n + 32 * ctas - 1) / (32 * ctas)));
+    for (int i = tid; i < used * experts; i += kSortThreads) lines[i] = 0;
     __syncthreads();
 
-    const int stretch = (pairs_n + ctas * kSortWarps - 1) / (ctas * kSortWarps);
-    const int64_t first = int64_t(cta * kSortWarps + warp) * stretch;
+    const int stretch = (pairs_n + ctas * used - 1) / (ctas * used);
+    const int64_t first = warp < used ? int64_t(cta * used + warp) * stretch : pairs_n;
     const int begin = int(min(first, int64_t(pairs_n))), end = int(min(first + stretch, int64_t(pairs_n)));
     int* const line = lines + warp * experts;
     for (int p = begin + lane; p < end; p += 32) {
@@ -72,7 +74,7 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const Id* __rest
     // a thread per expert (experts <= threads)
     if (tid < experts) {
         int sum = 0;
-        for (int w = 0; w < kSortWarps; ++w) {
+        for (int w = 0; w < used; ++w) {
             const int c = lines[w * experts + tid];
             lines[w * experts + tid] = sum;
             sum += c;
@@ -123,7 +125,7 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const Id* __rest
         count[tid] = all;
         start[tid] = run;
         if (tid == experts - 1) start[experts] = run + padded;
-        for (int w = 0; w < kSortWarps; ++w) lines[w * experts + tid] += run + before;
+        for (int w = 0; w < used; ++w) lines[w * experts + tid] += run + before;
         if (cta == 0) {
             offsets[tid] = run;
             if (tid == experts - 1) offsets[experts] = run + padded;
