@@ -10,8 +10,8 @@
 //   warps 0-7  promotion: tcgen05.ld of a block's sums, accumulators += scale * sums (two columns an instruction); after the last
 //              block the accumulators are rounded once and stored.  A thread has one row and half of the tile's columns.
 //   warp 8     TMA producer: A and B tiles (128-byte swizzle) into a ring of stages
-//   warps 9, 11  issue the MMAs of a block into the next of 2 (BN = 256) or 4 buffers of tensor memory, every other block each
-//   warp 10    brings the scales of four blocks at a time into shared memory, multiplied where a row has one factor per block
+//   warps 10, 11  issue the MMAs of a step (BN = 256: one block; else two, one each) into the next of 2 sets of buffers in tensor memory
+//   warp 9     brings the scales of four blocks at a time into shared memory, multiplied where a row has one factor per block
 //
 // Every mbarrier wait is bounded, as in the other GEMM kernels: a role that waits longer than kTimeoutNs records a code in the
 // status word, raises the CTA's abort flag and all roles leave through the common teardown.
@@ -64,9 +64,12 @@ struct BlockCfg {
     // a k-tile's scales: per row of the tile one for each of its blocks of weights (the product of both), or (kRowScales) the rows' and then the columns'
     static constexpr int kScales = kRowScales ? kTileM + BN : kTileM * kWeightBlocks;
     static constexpr int kScaleBytes = kScaleSlots * kGroupK * kScales * 4;
-    static constexpr int kExtra = kBarBytes + kTableBytes + kScaleBytes + 1024;
+    // a warp's finished 32 x 32 values on their way to a TMA store; all of a 256-wide tile's at a time
+    static constexpr int kEpiSlots = kRowScales ? 0 : BN == 256 ? 4 : 1;
+    static constexpr int kEpiBytes = kPromoWarps * kEpiSlots * 2048;
+    static constexpr int kExtra = kBarBytes + kTableBytes + kScaleBytes + kEpiBytes + 1024;
     static constexpr int kFit = (kSmemBudget - kExtra) / kStageBytes;
-    static constexpr int kStages = kStep == 1 ? kFit / 2 * 2 : kFit;
+    static constexpr int kStages = kFit;
     static constexpr int kSmemBytes = kStages * kStageBytes + kExtra;
     static constexpr int kBufs = 2;  // of kStep accumulators each
     static constexpr int kTmemCols = kBufs * kStep * BN;
@@ -75,7 +78,6 @@ struct BlockCfg {
     static constexpr int kThreads = (kPromoWarps + 4) * 32;
     // BN = 256: 128 accumulators a thread; the third warpgroup gives registers to the other two (168 * 384 = 208 * 256 + 88 * 128)
     static constexpr bool kRegSplit = BN == 256;
-    static_assert(kStep == 2 || (kStages % 2 == 0 && kBufs % 2 == 0), "each stage and buffer belongs to one MMA issuer");
     static_assert(sizeof(BlockBars) <= kBarBytes && kStages >= 3 && kStages <= 8 && kTmemCols <= 512, "budgets");
     static_assert(kTileM * (BN + 4) * 4 <= kStages * kStageBytes, "split-K partial sums fit into the ring");
 };
@@ -92,6 +94,7 @@ struct BlockArgs {
     int box_rows;   // rows of `a` per copy
     int out_type;   // HQ_DTYPE_*
     int out_align;  // 32, 16 or less: bytes that every row of the output starts on
+    int staged;     // 16-bit output that TMA can store
     int split;      // CTAs of a cluster that share a tile's k-tiles
     int wide_scales;  // both operands' scales are on 16 bytes
     int pdl;
@@ -294,16 +297,18 @@ __device__ __forceinline__ void store_values(const float (&f)[kN], void* out, in
 
 template <int BN, bool kRowScales, bool kGrouped, bool kSplit>
 __global__ void __launch_bounds__((BlockCfg<BN, kRowScales>::kThreads), 1)
-block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ BlockArgs p) {
+block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_d,
+                  const __grid_constant__ BlockArgs p) {
     using C = BlockCfg<BN, kRowScales>;
     extern __shared__ __align__(16) uint8_t smem_raw[];
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t a_base = ptx::smem_u32(smem);
     const uint32_t b_base = a_base + C::kStages * C::kStep * C::kABytes;
-    constexpr int kBarOffset = C::kStages * C::kStageBytes;
+    constexpr int kBarOffset = C::kStages * C::kStageBytes + C::kEpiBytes;
     BlockBars* const bars = reinterpret_cast<BlockBars*>(smem + kBarOffset);
     int* const tables = reinterpret_cast<int*>(smem + kBarOffset + C::kBarBytes);
     float* const scales = reinterpret_cast<float*>(smem + kBarOffset + C::kBarBytes + C::kTableBytes);
+    const uint32_t epi_base = a_base + C::kStages * C::kStageBytes;
     volatile uint32_t* const abort = &bars->abort;
     const int warp = warp_index();
     const int lane = threadIdx.x & 31;
@@ -325,6 +330,7 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         ptx::fence_mbar_init();
         ptx::prefetch_tmap(&tm_a);
         ptx::prefetch_tmap(&tm_b);
+        if (p.staged != 0) ptx::prefetch_tmap(&tm_d);
     }
     if (warp == kMmaWarp) {
         ptx::tmem_alloc<1>(ptx::smem_u32(&bars->tmem_base), C::kTmemCols);
@@ -420,14 +426,13 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         for (uint32_t d = it > uint32_t(C::kStages) ? it - C::kStages : 0u; ok && d < it; ++d) {
             ok = wait_bar<C::kRegSplit>(ptx::smem_u32(&bars->empty[d % C::kStages]), (d / C::kStages) & 1u, abort, kStatusProducer);
         }
-    } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
+    } else if (warp >= kMmaWarp && warp < kMmaWarp + C::kStep) {
         // ------------------------------------------------------------ MMA issuers
-        // Every k-tile has a buffer of its own, so nothing has to be kept in order between the two.  Steps of two: a k-tile of every step each.
-        // Steps of one: every other step each; stages and buffers are then even in number, so that each belongs to one issuer, which waits
-        // for all of its phases in turn (one that skipped a phase would find the wait for the next but one over before it began).
+        // One for each k-tile of a step.  Every k-tile has a buffer of its own, so nothing has to be kept in order between them.  (Two that took
+        // turns at the steps would skip phases of the stages' barriers, and a wait for the next but one is over before it began.)
         // float32 sums, e4m3 operands, both K-major; N >> 3, M >> 4
         constexpr uint32_t idesc = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(kTileM >> 4) << 24);
-        const uint32_t mine = warp == kMmaWarp ? 0u : 1u;
+        const uint32_t u = warp - kMmaWarp;
         const uint64_t adesc0 = ptx::smem_desc(a_base, 16, 1024, 2), bdesc0 = ptx::smem_desc(b_base, 16, 1024, 2);
         uint32_t it = 0;
         bool ok = true;
@@ -435,8 +440,7 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         BlockTile t;
         while (ok && walk.next(t)) {
             for (int kt = k_begin; kt < k_end; kt += C::kStep, ++it) {
-                if (C::kStep == 1 && (it & 1u) != mine) continue;
-                const uint32_t s = it % C::kStages, buf = it % C::kBufs, u = C::kStep == 1 ? 0u : mine;
+                const uint32_t s = it % C::kStages, buf = it % C::kBufs;
                 ok = wait_bars<C::kRegSplit>(ptx::smem_u32(&bars->full[s]), (it / C::kStages) & 1u, true, ptx::smem_u32(&bars->acc_empty[buf]),
                                ((it / C::kBufs) & 1u) ^ 1u, abort, kStatusMma);
                 if (!ok) break;
@@ -637,6 +641,34 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
                         }
                     }
                 }
+            } else if (p.staged != 0 && (kGrouped ? quarter * 32 + 32 <= t.valid : busy)) {
+                // 32 x 32 values at a time (rows and columns that are not there are dropped by the store; a run's last rows go the other way).
+                // 16-byte piece j of row r is at piece j ^ (r >> 1 & 3), the 64-byte swizzle of the tensor map.
+                const uint32_t slots = epi_base + warp * (C::kEpiSlots * 2048);
+#pragma unroll
+                for (int c = 0; c < C::kCols; c += 32) {
+                    const int col = t.n0 + part * C::kCols + c;
+                    if (col >= p.n) break;
+                    const uint32_t slot = slots + c / 32 % C::kEpiSlots * 2048;
+                    // the store that last read this slot (of this tile, or the one before) is done with it
+                    if (lane == 0) ptx::bulk_wait_read<C::kEpiSlots - 1>();
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int l = 0; l < 4; ++l) w[l] = pack16(acc[c + j * 8 + 2 * l], acc[c + j * 8 + 2 * l + 1], p.out_type);
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(slot + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)), "r"(w[0]),
+                                     "r"(w[1]), "r"(w[2]), "r"(w[3])
+                                     : "memory");
+                    }
+                    ptx::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        ptx::tma_store_2d(&tm_d, slot, col, t.row0 + quarter * 32);
+                        ptx::bulk_commit();
+                    }
+                }
             } else if (row_ok) {
                 const int col = t.n0 + part * C::kCols;
                 const int64_t at = int64_t(t.row0 + row) * p.ldo + col;
@@ -651,6 +683,9 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
             }
         }
     }
+
+    if (!kSplit && !kRowScales && warp < kPromoWarps && lane == 0) ptx::bulk_wait<0>();
+    __syncwarp();
 
     if constexpr (kSplit) {
         // One tile per cluster: every CTA adds up its share of the tile over the CTAs, in their order.
@@ -719,20 +754,26 @@ int launch_block_gemm(const BlockProblem& g, char* err, size_t errlen) {
     BlockArgs p = g.args;
     p.tiles_m = int((g.rows_a + kTileM - 1) / kTileM);
     p.tiles_n = int((g.n + BN - 1) / BN);
-    CUtensorMap tm_a, tm_b;
+    CUtensorMap tm_a, tm_b, tm_d;
     if (!make_tmap_2d(&tm_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.a, uint64_t(g.k), uint64_t(g.rows_a), uint64_t(g.k), kBlockK,
                       uint32_t(p.box_rows), CU_TENSOR_MAP_SWIZZLE_128B) ||
         !make_tmap_2d(&tm_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.b, uint64_t(g.k), uint64_t(g.n * g.experts), uint64_t(g.k), kBlockK, BN,
                       CU_TENSOR_MAP_SWIZZLE_128B)) {
         return fail(err, errlen, HQ_ERR_CUDA, "cuTensorMapEncodeTiled failed for the GEMM operands");
     }
+    // 16-bit results in whole pieces of 16 bytes leave through TMA (it stores a piece that the tensor ends in as a whole); others from
+    // registers, and another map stands in
+    p.staged = !kSplit && !kRowScales && p.out_type != HQ_DTYPE_FP32 && p.out_align >= 16 && g.n % 8 == 0 &&
+               make_tmap_2d(&tm_d, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.out, uint64_t(g.n), uint64_t(g.rows_a), uint64_t(p.ldo) * 2, 32, 32,
+                            CU_TENSOR_MAP_SWIZZLE_64B);
+    if (p.staged == 0) tm_d = tm_a;
     // grouped: a run may add a tile to those that its rows fill
     const int64_t row_tiles = kGrouped ? std::min<int64_t>(g.rows_a, g.rows_a / kTileM + g.experts) : p.tiles_m;
     const int64_t tiles = row_tiles * p.tiles_n;
     if (!kSplit) p.split = 1;
     const int64_t grid = kSplit ? tiles * p.split : std::min<int64_t>(tiles, g.sms);
     HQ_CUDA_TRY(launch(kernel, dim3(unsigned(grid)), dim3(C::kThreads), size_t(C::kSmemBytes), g.stream, p.pdl != 0,
-                       kSplit ? unsigned(p.split) : 1u, tm_a, tm_b, p));
+                       kSplit ? unsigned(p.split) : 1u, tm_a, tm_b, tm_d, p));
     return HQ_OK;
 }
 
