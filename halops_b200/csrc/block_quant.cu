@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(kRowThreads) swiglu_block_quant_kernel(const T
 
 // ---------------------------------------------------------------------------- gathered tokens
 //
-// A CTA reads and quantises 2048 values of one token once and writes them to each of the token's rows.  The blocks
+// A CTA reads and quantises 4096 values of one token, 16 a thread, once and writes them to each of the token's rows.  The blocks
 // behind the tokens write the rows that pad the experts' runs as the codes of zeros.
 
 template <typename T>
@@ -114,28 +114,32 @@ __global__ void __launch_bounds__(kRowThreads) permute_block_quant_kernel(const 
     grid_wait();
     grid_launch_dependents();
     const int kb = (k + kQBlock - 1) / kQBlock;
-    const int c = blockIdx.y * (kRowThreads * 8) + threadIdx.x * 8;
+    const int c = blockIdx.y * (kRowThreads * 16) + threadIdx.x * 16;
     if (int(blockIdx.x) >= tokens) {
         const int e = int(blockIdx.x) - tokens;
         const BlockScale s = block_scale(0, true);
         for (int r = min(offsets[e + 1], n_rows) - 1; r >= max(offsets[e], 0) && pairs[r] < 0; --r) {
             if (c < k) {
-                *reinterpret_cast<uint2*>(q + int64_t(r) * k + c) = make_uint2(0, 0);
-                if ((threadIdx.x & 15) == 0) sf[int64_t(r) * kb + c / kQBlock] = s.scale;
+                *reinterpret_cast<uint4*>(q + int64_t(r) * k + c) = make_uint4(0, 0, 0, 0);
+                if ((threadIdx.x & 7) == 0) sf[int64_t(r) * kb + c / kQBlock] = s.scale;
             }
         }
         return;
     }
     const int64_t token = blockIdx.x;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (c < k) v = load_stream(x + token * ld + c);
-    const BlockScale s = block_scale(magnitude_f32<T>(max16(amax16(v))), true);
-    const uint2 code = codes8<T>(v, s);
+    uint4 v = make_uint4(0, 0, 0, 0), w = v;
+    if (c < k) v = load_stream(x + token * ld + c), w = load_stream(x + token * ld + c + 8);
+    uint32_t amax = max(amax16(v), amax16(w));
+#pragma unroll
+    for (int d = 1; d < 8; d *= 2) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+    const BlockScale s = block_scale(magnitude_f32<T>(amax), true);
+    const uint2 lo = codes8<T>(v, s), hi = codes8<T>(w, s);
+    if (c >= k) return;
     for (int j = 0; j < topk; ++j) {
         const int r = __ldg(rows + token * topk + j);
-        if (r >= 0 && r < n_rows && c < k) {
-            *reinterpret_cast<uint2*>(q + int64_t(r) * k + c) = code;
-            if ((threadIdx.x & 15) == 0) sf[int64_t(r) * kb + c / kQBlock] = s.scale;
+        if (r >= 0 && r < n_rows) {
+            *reinterpret_cast<uint4*>(q + int64_t(r) * k + c) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            if ((threadIdx.x & 7) == 0) sf[int64_t(r) * kb + c / kQBlock] = s.scale;
         }
     }
 }
@@ -381,7 +385,7 @@ extern "C" int hq_moe_permute_block_quant(const void* input, int64_t ld_elems, i
     }
     const hq::DeviceGuard guard(device);
     if (!guard.ok()) return fail(err, errlen, HQ_ERR_CUDA, "cannot select CUDA device %d", device);
-    const dim3 grid(unsigned(tokens + (padded != 0 ? num_experts : 0)), unsigned((k + hq::kRowThreads * 8 - 1) / (hq::kRowThreads * 8)));
+    const dim3 grid(unsigned(tokens + (padded != 0 ? num_experts : 0)), unsigned((k + hq::kRowThreads * 16 - 1) / (hq::kRowThreads * 16)));
     const auto go = [&](auto kernel, auto* x) {
         return hq::launch(kernel, grid, dim3(hq::kRowThreads), 0, static_cast<cudaStream_t>(stream), use_pdl != 0, 1, x, ld_elems,
                           int(tokens), int(k), int(topk), rows, pairs, offsets, int(n_rows), static_cast<uint8_t*>(out_q),

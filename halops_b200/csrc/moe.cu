@@ -52,7 +52,8 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const Id* __rest
     int* const lines = smem;                             // [warp][expert]
     int* const total = lines + kSortWarps * experts;     // this CTA's pairs per expert, read by the cluster
     int* const count = total + experts;                  // all pairs per expert
-    int* const start = count + experts;                  // first row of the expert's run, and the end of the last
+    int* const base = count + experts;                   // row of this CTA's first pair of the expert
+    int* const start = base + experts;                   // first row of the expert's run, and the end of the last
     __shared__ int warp_sums[kSortWarps];
     grid_wait();
     grid_launch_dependents();
@@ -66,18 +67,32 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const Id* __rest
     const int64_t first = warp < used ? int64_t(cta * used + warp) * stretch : pairs_n;
     const int begin = int(min(first, int64_t(pairs_n))), end = int(min(first + stretch, int64_t(pairs_n)));
     int* const line = lines + warp * experts;
-    for (int p = begin + lane; p < end; p += 32) {
+    // the first pairs' experts stay in registers for the second pass, and are all asked for before the first is counted
+    constexpr int kHeld = 8;
+    int held[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) held[i] = expert_of(ids, begin + i * 32 + lane, end, experts);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+        if (held[i] >= 0) atomicAdd(line + held[i], 1);
+    }
+    for (int p = begin + kHeld * 32 + lane; p < end; p += 32) {
         const int e = expert_of(ids, p, end, experts);
         if (e >= 0) atomicAdd(line + e, 1);
     }
     __syncthreads();
-    // a thread per expert (experts <= threads)
+    // a thread per expert (experts <= threads): exclusive sums over the lines, eight of which are read at a time
     if (tid < experts) {
         int sum = 0;
-        for (int w = 0; w < used; ++w) {
-            const int c = lines[w * experts + tid];
-            lines[w * experts + tid] = sum;
-            sum += c;
+        for (int w0 = 0; w0 < used; w0 += 8) {
+            int c[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) c[j] = w0 + j < used ? lines[(w0 + j) * experts + tid] : 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (w0 + j < used) lines[(w0 + j) * experts + tid] = sum;
+                sum += c[j];
+            }
         }
         total[tid] = sum;
     }
@@ -125,7 +140,7 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const Id* __rest
         count[tid] = all;
         start[tid] = run;
         if (tid == experts - 1) start[experts] = run + padded;
-        for (int w = 0; w < used; ++w) lines[w * experts + tid] += run + before;
+        base[tid] = run + before;
         if (cta == 0) {
             offsets[tid] = run;
             if (tid == experts - 1) offsets[experts] = run + padded;
@@ -133,27 +148,39 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const Id* __rest
     }
     __syncthreads();
 
-    for (int p0 = begin; p0 < end; p0 += 32) {
+    const auto place = [&](int p0, int e) {
         const int p = p0 + lane;
-        const int e = expert_of(ids, p, end, experts);
         const uint32_t same = __match_any_sync(0xffffffffu, e);
         int at = -1;
-        if (e >= 0) at = line[e] + __popc(same & ((1u << lane) - 1u));
+        int seen = 0;
+        if (e >= 0) seen = line[e], at = base[e] + seen + __popc(same & ((1u << lane) - 1u));
         __syncwarp();
-        if (e >= 0 && lane == 31 - __clz(same)) line[e] = at + 1;
+        if (e >= 0 && lane == 31 - __clz(same)) line[e] = seen + __popc(same);
         __syncwarp();
         if (p < end) rows[p] = at;
         if (at >= 0 && at < n_rows) pairs[at] = p;
+    };
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+        if (begin + i * 32 < end) place(begin + i * 32, held[i]);
     }
-    // the rows' experts, and the rows without a pair
-    for (int r = cta * kSortThreads + tid; r < n_rows; r += ctas * kSortThreads) {
-        int lo = 0, hi = experts;  // the last expert whose run starts at or before r (empty runs start where the next does)
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (start[mid] <= r) lo = mid; else hi = mid;
+    for (int p0 = begin + kHeld * 32; p0 < end; p0 += 32) place(p0, expert_of(ids, p0 + lane, end, experts));
+    // The rows' experts (the last whose run starts at or before a row: empty runs start where the next does), and the rows without a
+    // pair: where there are more rows than threads, four neighbouring ones a thread, of which only the first is searched for.
+    int top = 1;
+    while (top * 2 < experts) top *= 2;
+    const int per = n_rows > ctas * kSortThreads ? 4 : 1;
+    for (int64_t r0 = per * int64_t(cta * kSortThreads + tid); r0 < n_rows; r0 += per * ctas * kSortThreads) {
+        int e = 0;
+        for (int d = top; d > 0; d /= 2) {
+            if (e + d < experts && start[e + d] <= r0) e += d;
         }
-        expert_ids[r] = lo;
-        if (r - start[lo] >= count[lo]) pairs[r] = -1;
+        for (int i = 0; i < per && r0 + i < n_rows; ++i) {
+            const int r = int(r0) + i;
+            while (e + 1 < experts && start[e + 1] <= r) ++e;
+            expert_ids[r] = e;
+            if (r - start[e] >= count[e]) pairs[r] = -1;
+        }
     }
     __syncwarp();
     if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -189,12 +216,17 @@ __global__ void __launch_bounds__(kMoveThreads) moe_permute_kernel(const Unit* _
     for (int i = 0; i < kPer; ++i) {
         if (c + i * kMoveThreads < units) v[i] = x[token * ld + c + i * kMoveThreads];
     }
-    for (int j = 0; j < topk; ++j) {
-        const int r = __ldg(rows + token * topk + j);
-        if (r < 0 || r >= n_rows) continue;
+    for (int j0 = 0; j0 < topk; j0 += 8) {
+        int r[8];
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            if (c + i * kMoveThreads < units) out[int64_t(r) * units + c + i * kMoveThreads] = v[i];
+        for (int j = 0; j < 8; ++j) r[j] = j0 + j < topk ? __ldg(rows + token * topk + j0 + j) : -1;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (r[j] < 0 || r[j] >= n_rows) continue;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                if (c + i * kMoveThreads < units) out[int64_t(r[j]) * units + c + i * kMoveThreads] = v[i];
+            }
         }
     }
 }
@@ -290,7 +322,7 @@ struct Piece {
     }
 };
 
-template <typename T, bool kWide>
+template <typename T, bool kWide, int kPer>
 __global__ void __launch_bounds__(kMoveThreads) moe_unpermute_kernel(const T* __restrict__ z, int64_t ld, int tokens, int h, int topk,
                                                                      const int* __restrict__ rows, int n_rows,
                                                                      const float* __restrict__ weights, T* __restrict__ y) {
@@ -299,13 +331,17 @@ __global__ void __launch_bounds__(kMoveThreads) moe_unpermute_kernel(const T* __
     grid_wait();
     grid_launch_dependents();
     const int64_t token = blockIdx.x;
-    const int c = (blockIdx.y * kMoveThreads + threadIdx.x) * P::kN;
+    constexpr int kStep = kMoveThreads * P::kN;
+    const int c = blockIdx.y * (kStep * kPer) + threadIdx.x * P::kN;
     if (c >= h) return;
-    float sum[P::kN];
+    float sum[kPer][P::kN];
 #pragma unroll
-    for (int i = 0; i < P::kN; ++i) sum[i] = 0.0f;
+    for (int q = 0; q < kPer; ++q) {
+#pragma unroll
+        for (int i = 0; i < P::kN; ++i) sum[q][i] = 0.0f;
+    }
     for (int j0 = 0; j0 < topk; j0 += kSlots) {
-        P piece[kSlots];
+        P piece[kSlots][kPer];
         float w[kSlots];
         bool here[kSlots];
 #pragma unroll
@@ -315,98 +351,102 @@ __global__ void __launch_bounds__(kMoveThreads) moe_unpermute_kernel(const T* __
             here[j] = r >= 0 && r < n_rows;
             w[j] = 1.0f;
             if (here[j]) {
-                piece[j].load(z + int64_t(r) * ld + c);
+#pragma unroll
+                for (int q = 0; q < kPer; ++q) {
+                    if (c + q * kStep < h) piece[j][q].load(z + int64_t(r) * ld + c + q * kStep);
+                }
                 if (weights != nullptr) w[j] = __ldg(weights + token * topk + j0 + j);
             }
         }
 #pragma unroll
         for (int j = 0; j < kSlots; ++j) {
             if (!here[j]) continue;
-            float f[P::kN];
-            piece[j].get(f);
 #pragma unroll
-            for (int i = 0; i < P::kN; ++i) sum[i] = fmaf(w[j], f[i], sum[i]);
+            for (int q = 0; q < kPer; ++q) {
+                if (c + q * kStep >= h) continue;
+                float f[P::kN];
+                piece[j][q].get(f);
+#pragma unroll
+                for (int i = 0; i < P::kN; ++i) sum[q][i] = fmaf(w[j], f[i], sum[q][i]);
+            }
         }
     }
-    P::store(y + token * h + c, sum);
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+        if (c + q * kStep < h) P::store(y + token * h + c + q * kStep, sum[q]);
+    }
 }
 
-// The gradients of the above: gz[row] = weight * gy[token], gw[pair] = <gy[token], z[row]>.  A CTA has one token, whose
-// gradient stays in registers (up to kKeep pieces a thread, the rest is read again per slot); the CTAs behind the tokens zero the rows
-// that pad the runs.
-template <typename T, bool kWide>
+// The gradients of the above: gz[row] = weight * gy[token], gw[pair] = <gy[token], z[row]>.  A group of kGroup threads has one pair
+// (a warp; a whole CTA where there are few pairs), with kAhead pieces of both rows in flight per thread; the pairs of a token are
+// neighbours, so that its gradient comes from HBM once.  The CTAs behind the pairs zero the rows that pad the runs.
+template <typename T, bool kWide, int kGroup>
 __global__ void __launch_bounds__(kMoveThreads) moe_unpermute_backward_kernel(
-    const T* __restrict__ gy, int64_t ld_g, const T* __restrict__ z, int64_t ld_z, int tokens, int h, int topk, const int* __restrict__ rows,
-    const int* __restrict__ pairs, const int* __restrict__ offsets, int n_rows, const float* __restrict__ weights, T* __restrict__ gz,
-    float* __restrict__ gw) {
+    const T* __restrict__ gy, int64_t ld_g, const T* __restrict__ z, int64_t ld_z, int pairs_n, int pair_ctas, int h, int topk,
+    const int* __restrict__ rows, const int* __restrict__ pairs, const int* __restrict__ offsets, int n_rows,
+    const float* __restrict__ weights, T* __restrict__ gz, float* __restrict__ gw) {
     using P = Piece<T, kWide>;
-    constexpr int kKeep = 2, kStep = kMoveThreads * P::kN;
-    __shared__ float parts[2][kMoveThreads / 32];
+    constexpr int kAhead = 4, kStep = kGroup * P::kN;
+    __shared__ float parts[kMoveThreads / 32];
     grid_wait();
     grid_launch_dependents();
-    const int c0 = threadIdx.x * P::kN;
-    if (int(blockIdx.x) >= tokens) {
-        const int e = int(blockIdx.x) - tokens;
+    if (int(blockIdx.x) >= pair_ctas) {
+        const int e = int(blockIdx.x) - pair_ctas;
         float zero[P::kN];
 #pragma unroll
         for (int i = 0; i < P::kN; ++i) zero[i] = 0.0f;
         for (int r = min(offsets[e + 1], n_rows) - 1; r >= max(offsets[e], 0) && pairs[r] < 0; --r) {
-            for (int c = c0; c < h; c += kStep) P::store(gz + int64_t(r) * h + c, zero);
+            for (int c = threadIdx.x * P::kN; c < h; c += kMoveThreads * P::kN) P::store(gz + int64_t(r) * h + c, zero);
         }
         return;
     }
-    const int64_t token = blockIdx.x;
-    const T* const g = gy + token * ld_g;
-    P kept[kKeep];
+    const int64_t pair = int64_t(blockIdx.x) * (kMoveThreads / kGroup) + threadIdx.x / kGroup;
+    if (pair >= pairs_n) return;  // (whole groups)
+    const int r = __ldg(rows + pair);
+    const bool here = r >= 0 && r < n_rows;
+    float dot = 0.0f;
+    if (here) {
+        const T* const g = gy + pair / topk * ld_g;
+        const T* const s = z + int64_t(r) * ld_z;
+        T* const to = gz + int64_t(r) * h;
+        const float w = weights != nullptr ? __ldg(weights + pair) : 1.0f;
+        for (int c0 = (threadIdx.x % kGroup) * P::kN; c0 < h; c0 += kAhead * kStep) {
+            P a[kAhead], b[kAhead];
 #pragma unroll
-    for (int i = 0; i < kKeep; ++i) {
-        if (c0 + i * kStep < h) kept[i].load(g + c0 + i * kStep);
+            for (int i = 0; i < kAhead; ++i) {
+                if (c0 + i * kStep < h) {
+                    a[i].load(g + c0 + i * kStep);
+                    if (gw != nullptr) b[i].load(s + c0 + i * kStep);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                if (c0 + i * kStep >= h) continue;
+                float f[P::kN], o[P::kN];
+                a[i].get(f);
+                if (gw != nullptr) {
+                    float u[P::kN];
+                    b[i].get(u);
+#pragma unroll
+                    for (int j = 0; j < P::kN; ++j) dot = fmaf(f[j], u[j], dot);
+                }
+#pragma unroll
+                for (int j = 0; j < P::kN; ++j) o[j] = w * f[j];
+                P::store(to + c0 + i * kStep, o);
+            }
+        }
     }
-    for (int j = 0; j < topk; ++j) {
-        const int r = __ldg(rows + token * topk + j);  // the same for the whole CTA
-        if (r < 0 || r >= n_rows) {
-            if (gw != nullptr && threadIdx.x == 0) gw[token * topk + j] = 0.0f;
-            continue;
-        }
-        const float w = weights != nullptr ? __ldg(weights + token * topk + j) : 1.0f;
-        float dot = 0.0f;
-        const auto piece = [&](const P& p, int c) {
-            float f[P::kN], o[P::kN];
-            p.get(f);
+    if (gw != nullptr) {
 #pragma unroll
-            for (int i = 0; i < P::kN; ++i) o[i] = w * f[i];
-            if (gw != nullptr) {
-                P s;
-                s.load(z + int64_t(r) * ld_z + c);
-                float u[P::kN];
-                s.get(u);
-#pragma unroll
-                for (int i = 0; i < P::kN; ++i) dot = fmaf(f[i], u[i], dot);
-            }
-            P::store(gz + int64_t(r) * h + c, o);
-        };
-#pragma unroll
-        for (int i = 0; i < kKeep; ++i) {
-            if (c0 + i * kStep < h) piece(kept[i], c0 + i * kStep);
-        }
-        for (int c = c0 + kKeep * kStep; c < h; c += kStep) {
-            P p;
-            p.load(g + c);
-            piece(p, c);
-        }
-        if (gw != nullptr) {
-#pragma unroll
-            for (int d = 16; d > 0; d /= 2) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-            // two sets of sums, used in turn: a set is written again only behind the next slot's barrier
-            if ((threadIdx.x & 31) == 0) parts[j & 1][threadIdx.x >> 5] = dot;
+        for (int d = 16; d > 0; d /= 2) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+        if constexpr (kGroup > 32) {
+            if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = dot;
             __syncthreads();
-            if (threadIdx.x == 0) {
-                float sum = 0.0f;
+            dot = 0.0f;
 #pragma unroll
-                for (int i = 0; i < kMoveThreads / 32; ++i) sum += parts[j & 1][i];
-                gw[token * topk + j] = sum;
-            }
+            for (int i = 0; i < kMoveThreads / 32; ++i) dot += parts[i];
         }
+        if (threadIdx.x % kGroup == 0) gw[pair] = dot;
     }
 }
 
@@ -419,17 +459,19 @@ template <typename Id>
 cudaError_t launch_sort(const void* ids, int pairs_n, int experts, int align, int n_rows, bool pdl, int* rows, int* pairs, int* offsets,
                         int* expert_ids, cudaStream_t stream) {
     static SortOptIn opt;
-    // One CTA goes over 128 pairs a warp in 4 steps; from there on 8 CTAs repay the two barriers of their cluster.
-    const int ctas = pairs_n > 4096 || n_rows > 16384 ? 8 : 1;
-    const int bytes = int(sizeof(int)) * ((kSortWarps + 3) * experts + 1);
-    if (bytes > 40 * 1024) {
+    // One CTA goes over 128 pairs a warp in 4 steps; from there on 8 CTAs repay the two barriers of their cluster, and 16 (which a kernel
+    // has to opt in to) where there are thousands of pairs for each: 65536 pairs 15.2 -> 11.8 us, 32768 9.6 -> 8.5.
+    const int ctas = pairs_n > 16384 ? 16 : pairs_n > 4096 || n_rows > 16384 ? 8 : 1;
+    const auto need = [](int e) { return int(sizeof(int)) * (kSortWarps * e + 4 * e + 1); };
+    const int bytes = need(experts);
+    if (bytes > 40 * 1024 || ctas > 8) {
         int dev = 0;
         const cudaError_t e = cudaGetDevice(&dev);
         if (e != cudaSuccess) return e;
         const std::lock_guard<std::mutex> lock(opt.mu);
         if (dev < 0 || dev >= 64 || opt.done[dev] == 0) {
-            const int most = int(sizeof(int)) * ((kSortWarps + 3) * kMaxExperts + 1);
-            const cudaError_t f = cudaFuncSetAttribute(moe_sort_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+            cudaError_t f = cudaFuncSetAttribute(moe_sort_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, need(kMaxExperts));
+            if (f == cudaSuccess) f = cudaFuncSetAttribute(moe_sort_kernel<Id>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
             if (f != cudaSuccess) return f;
             if (dev >= 0 && dev < 64) opt.done[dev] = 1;
         }
@@ -534,7 +576,10 @@ extern "C" int hq_moe_unpermute(const void* input, int64_t ld_elems, int dtype, 
     const hq::DeviceGuard guard(device);
     if (!guard.ok()) return fail(err, errlen, HQ_ERR_CUDA, "cannot select CUDA device %d", device);
     const bool wide = hq::aligned(input, 16) && hq::aligned(output, 16) && ld_elems * size % 16 == 0 && h * size % 16 == 0;
-    const int64_t per = hq::kMoveThreads * int64_t(wide ? 16 / size : 1);
+    // two pieces a thread where rows fill them and there are tokens for all SMs: more bytes in flight per CTA
+    const int64_t one = hq::kMoveThreads * int64_t(wide ? 16 / size : 1);
+    const bool two = wide && h >= 2 * one && tokens >= 1024;
+    const int64_t per = two ? 2 * one : one;
     const dim3 grid(unsigned(tokens), unsigned((h + per - 1) / per));
     const auto go = [&](auto kernel, auto* z) {
         using T = std::remove_const_t<std::remove_pointer_t<decltype(z)>>;
@@ -543,7 +588,9 @@ extern "C" int hq_moe_unpermute(const void* input, int64_t ld_elems, int dtype, 
     };
     const auto typed = [&](auto* z) {
         using T = std::remove_const_t<std::remove_pointer_t<decltype(z)>>;
-        return wide ? go(hq::moe_unpermute_kernel<T, true>, z) : go(hq::moe_unpermute_kernel<T, false>, z);
+        return !wide ? go(hq::moe_unpermute_kernel<T, false, 1>, z)
+               : two ? go(hq::moe_unpermute_kernel<T, true, 2>, z)
+                     : go(hq::moe_unpermute_kernel<T, true, 1>, z);
     };
     HQ_CUDA_TRY(dtype == HQ_DTYPE_BF16   ? typed(static_cast<const __nv_bfloat16*>(input))
                 : dtype == HQ_DTYPE_FP16 ? typed(static_cast<const __half*>(input))
@@ -570,16 +617,21 @@ extern "C" int hq_moe_unpermute_backward(const void* grad_output, int64_t ld_gra
     if (!guard.ok()) return fail(err, errlen, HQ_ERR_CUDA, "cannot select CUDA device %d", device);
     const bool wide = hq::aligned(grad_output, 16) && hq::aligned(grad_input, 16) && hq::aligned(input, 16) && ld_grad * size % 16 == 0 &&
                       ld_input * size % 16 == 0 && h * size % 16 == 0;
-    const dim3 grid(unsigned(tokens + (padded != 0 ? num_experts : 0)));
+    // a warp per pair once they fill the SMs (148 of 16 CTAs' warps), else a CTA
+    const int64_t n = tokens * topk;
+    const bool warps = n >= 148 * 16;
+    const int64_t pair_ctas = warps ? (n + hq::kMoveThreads / 32 - 1) / (hq::kMoveThreads / 32) : n;
+    const dim3 grid(unsigned(pair_ctas + (padded != 0 ? num_experts : 0)));
     const auto go = [&](auto kernel, auto* g) {
         using T = std::remove_const_t<std::remove_pointer_t<decltype(g)>>;
         return hq::launch(kernel, grid, dim3(hq::kMoveThreads), 0, static_cast<cudaStream_t>(stream), use_pdl != 0, 1, g, ld_grad,
-                          static_cast<const T*>(input), ld_input, int(tokens), int(h), int(topk), rows, pairs, offsets, int(n_rows), weights,
+                          static_cast<const T*>(input), ld_input, int(n), int(pair_ctas), int(h), int(topk), rows, pairs, offsets, int(n_rows), weights,
                           static_cast<T*>(grad_input), grad_weights);
     };
     const auto typed = [&](auto* g) {
         using T = std::remove_const_t<std::remove_pointer_t<decltype(g)>>;
-        return wide ? go(hq::moe_unpermute_backward_kernel<T, true>, g) : go(hq::moe_unpermute_backward_kernel<T, false>, g);
+        return wide ? (warps ? go(hq::moe_unpermute_backward_kernel<T, true, 32>, g) : go(hq::moe_unpermute_backward_kernel<T, true, hq::kMoveThreads>, g))
+                    : (warps ? go(hq::moe_unpermute_backward_kernel<T, false, 32>, g) : go(hq::moe_unpermute_backward_kernel<T, false, hq::kMoveThreads>, g));
     };
     HQ_CUDA_TRY(dtype == HQ_DTYPE_BF16   ? typed(static_cast<const __nv_bfloat16*>(grad_output))
                 : dtype == HQ_DTYPE_FP16 ? typed(static_cast<const __half*>(grad_output))
