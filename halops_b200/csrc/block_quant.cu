@@ -18,8 +18,15 @@ __device__ __forceinline__ uint4 load_stream(const void* p) {
 
 // ---------------------------------------------------------------------------- rows
 //
-// A lane holds 8 neighbouring values, 16 lanes a block; a warp has kVec pieces of 256 values of one row, all
-// loaded before the first is worked on.
+// A lane holds 16 neighbouring values, 8 lanes a block; a warp has kVec pieces of 512 values of one row, all
+// loaded before the first is worked on.  (With 8 values a lane and 8-byte stores of codes 8192 x 8192 took 39.3 us, so 33.3.)
+
+// Maximum over the 8 lanes that hold a block.
+__device__ __forceinline__ uint32_t max8(uint32_t m) {
+#pragma unroll
+    for (int d = 1; d < 8; d *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+    return m;
+}
 
 template <typename T, int kVec>
 __global__ void __launch_bounds__(kRowThreads) block_quant_rows_kernel(const T* __restrict__ x, int64_t ld, int64_t m, int k, int segs,
@@ -30,22 +37,23 @@ __global__ void __launch_bounds__(kRowThreads) block_quant_rows_kernel(const T* 
     const int64_t task = int64_t(blockIdx.x) * (kRowThreads / 32) + (threadIdx.x >> 5);
     const int64_t row = task / segs;
     if (row >= m) return;
-    const int col = int(task - row * segs) * (kVec * 256) + lane * 8;
+    const int col = int(task - row * segs) * (kVec * 512) + lane * 16;
     const int kb = (k + kQBlock - 1) / kQBlock;
     const T* const src = x + row * ld + col;
-    uint4 v[kVec];
+    uint4 v[kVec][2];
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
-        v[i] = make_uint4(0, 0, 0, 0);
-        if (col + i * 256 < k) v[i] = load_stream(src + i * 256);
+        v[i][0] = v[i][1] = make_uint4(0, 0, 0, 0);
+        if (col + i * 512 < k) v[i][0] = load_stream(src + i * 512), v[i][1] = load_stream(src + i * 512 + 8);
     }
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
-        const int c = col + i * 256;
-        const BlockScale s = block_scale(magnitude_f32<T>(max16(amax16(v[i]))), true);
+        const int c = col + i * 512;
+        const BlockScale s = block_scale(magnitude_f32<T>(max8(max(amax16(v[i][0]), amax16(v[i][1])))), true);
         if (c < k) {
-            *reinterpret_cast<uint2*>(q + row * k + c) = codes8<T>(v[i], s);
-            if ((lane & 15) == 0) sf[row * kb + c / kQBlock] = s.scale;
+            const uint2 lo = codes8<T>(v[i][0], s), hi = codes8<T>(v[i][1], s);
+            *reinterpret_cast<uint4*>(q + row * k + c) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            if ((lane & 7) == 0) sf[row * kb + c / kQBlock] = s.scale;
         }
     }
 }
@@ -59,45 +67,43 @@ template <typename T>
 __global__ void __launch_bounds__(kRowThreads) swiglu_block_quant_kernel(const T* __restrict__ x, int64_t ld, int64_t m, int k, int segs,
                                                                          const int* __restrict__ row_limit, uint8_t* __restrict__ q,
                                                                          float* __restrict__ sf) {
-    constexpr int kVec = 2;
     grid_wait();
     grid_launch_dependents();
     const int lane = threadIdx.x & 31;
     const int64_t task = int64_t(blockIdx.x) * (kRowThreads / 32) + (threadIdx.x >> 5);
     const int64_t row = task / segs;
     if (row >= m || (row_limit != nullptr && row >= __ldg(row_limit))) return;
-    const int col = int(task - row * segs) * (kVec * 256) + lane * 8;
+    const int c = int(task - row * segs) * 512 + lane * 16;
     const int kb = (k + kQBlock - 1) / kQBlock;
-    const T* const src = x + row * ld + col;
-    uint4 gate[kVec], up[kVec];
+    const T* const src = x + row * ld + c;
+    uint4 gate[2], up[2];
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
+    for (int i = 0; i < 2; ++i) {
         gate[i] = up[i] = make_uint4(0, 0, 0, 0);
-        if (col + i * 256 < k) {
-            gate[i] = load_stream(src + i * 256);
-            up[i] = load_stream(src + k + i * 256);
-        }
+        if (c < k) gate[i] = load_stream(src + i * 8), up[i] = load_stream(src + k + i * 8);
     }
+    float2 h[8];
+    uint32_t amax = 0;
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-        const int c = col + i * 256;
+    for (int i = 0; i < 2; ++i) {
         const uint32_t gw[4] = {gate[i].x, gate[i].y, gate[i].z, gate[i].w}, uw[4] = {up[i].x, up[i].y, up[i].z, up[i].w};
-        float2 h[4];
-        uint32_t amax = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float2 g = two_floats<T>(gw[j]), u = two_floats<T>(uw[j]);
+            float2& o = h[i * 4 + j];
             // (__fdividef gives 0 for a divisor above 2^126, where the quotient is below 2^-119)
-            h[j].x = __fdividef(g.x, 1.0f + __expf(-g.x)) * u.x;
-            h[j].y = __fdividef(g.y, 1.0f + __expf(-g.y)) * u.y;
-            amax = max(amax, max(__float_as_uint(h[j].x) & 0x7fffffffu, __float_as_uint(h[j].y) & 0x7fffffffu));
+            o.x = __fdividef(g.x, 1.0f + __expf(-g.x)) * u.x;
+            o.y = __fdividef(g.y, 1.0f + __expf(-g.y)) * u.y;
+            amax = max(amax, max(__float_as_uint(o.x) & 0x7fffffffu, __float_as_uint(o.y) & 0x7fffffffu));
         }
-        const BlockScale s = block_scale(max16(amax), false);
-        if (c < k) {
-            *reinterpret_cast<uint2*>(q + row * k + c) =
-                make_uint2(code2(h[0], s) | code2(h[1], s) << 16, code2(h[2], s) | code2(h[3], s) << 16);
-            if ((lane & 15) == 0) sf[row * kb + c / kQBlock] = s.scale;
-        }
+    }
+    const BlockScale s = block_scale(max8(amax), false);
+    if (c < k) {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = code2(h[2 * j], s) | code2(h[2 * j + 1], s) << 16;
+        *reinterpret_cast<uint4*>(q + row * k + c) = make_uint4(w[0], w[1], w[2], w[3]);
+        if ((lane & 7) == 0) sf[row * kb + c / kQBlock] = s.scale;
     }
 }
 
@@ -129,10 +135,7 @@ __global__ void __launch_bounds__(kRowThreads) permute_block_quant_kernel(const 
     const int64_t token = blockIdx.x;
     uint4 v = make_uint4(0, 0, 0, 0), w = v;
     if (c < k) v = load_stream(x + token * ld + c), w = load_stream(x + token * ld + c + 8);
-    uint32_t amax = max(amax16(v), amax16(w));
-#pragma unroll
-    for (int d = 1; d < 8; d *= 2) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, d));
-    const BlockScale s = block_scale(magnitude_f32<T>(amax), true);
+    const BlockScale s = block_scale(magnitude_f32<T>(max8(max(amax16(v), amax16(w)))), true);
     const uint2 lo = codes8<T>(v, s), hi = codes8<T>(w, s);
     if (c >= k) return;
     for (int j = 0; j < topk; ++j) {
@@ -154,7 +157,8 @@ __global__ void __launch_bounds__(kRowThreads) permute_block_quant_kernel(const 
 template <typename T, bool kSquare, bool kTranspose>
 __global__ void __launch_bounds__(256) block_quant_tile_kernel(const T* __restrict__ x, int64_t ld, int64_t batch_stride, int64_t m, int k,
                                                                int64_t m_out, uint8_t* __restrict__ q, float* __restrict__ sf) {
-    __shared__ uint32_t amax_s[8][128];
+    __shared__ uint32_t amax_s[8][64];
+    __shared__ float2 factors[kSquare ? 1 : 128];  // of each column: 448 / amax, and whether its block is finite
     __shared__ __align__(16) uint8_t tile[kTranspose ? 128 * 128 : 16];
     grid_wait();
     grid_launch_dependents();
@@ -203,17 +207,22 @@ __global__ void __launch_bounds__(256) block_quant_tile_kernel(const T* __restri
             if (lane < 16) amax_s[warp][cg * 4 + j] = a[j];
         }
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        // a thread per column: the divisions are made once for its 16 readers
+        if (tid < 128) {
             uint32_t b = 0;
 #pragma unroll
-            for (int w = 0; w < 8; ++w) b = __vmaxu2(b, amax_s[w][cg * 4 + j]);
-            s[2 * j] = block_scale(magnitude_f32<T>(b & 0xffffu), true);
-            s[2 * j + 1] = block_scale(magnitude_f32<T>(b >> 16), true);
+            for (int w = 0; w < 8; ++w) b = __vmaxu2(b, amax_s[w][tid / 2]);
+            const BlockScale one = block_scale(magnitude_f32<T>(tid % 2 == 0 ? b & 0xffffu : b >> 16), true);
+            factors[tid] = make_float2(one.inverse, __uint_as_float(one.add));
+            if (col0 + tid < k) sf[int64_t(col0 + tid) * mb + blockIdx.x] = one.scale;
         }
-        if (rg == 0 && col < k) {
+        __syncthreads();
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sf[int64_t(col + j) * mb + blockIdx.x] = s[j].scale;
+        for (int j = 0; j < 8; ++j) {
+            const float2 f = factors[cg * 8 + j];
+            s[j].inverse = f.x;
+            s[j].add = __float_as_uint(f.y);
+            s[j].mask = s[j].add != 0 ? ~7u : ~0u;
         }
     }
     if constexpr (!kTranspose) {
@@ -265,12 +274,12 @@ cudaError_t launch_block_quant(const void* input, int64_t ld, int64_t batch_stri
     uint8_t* const oq = static_cast<uint8_t*>(q);
     float* const os = static_cast<float*>(sf);
     if (!square && !transpose) {
-        // Few rows: a piece of 256 values per warp, for more warps; else 4, for more bytes in flight per warp.
+        // Few rows: a piece of 512 values per warp, for more warps; else 2, for more bytes in flight per warp.
         const bool few = m * k < (int64_t(1) << 20);
-        const int segs = (k + (few ? 255 : 1023)) / (few ? 256 : 1024);
+        const int segs = (k + (few ? 511 : 1023)) / (few ? 512 : 1024);
         const dim3 grid(unsigned((m * segs + kRowThreads / 32 - 1) / (kRowThreads / 32)));
         return few ? launch(block_quant_rows_kernel<T, 1>, grid, dim3(kRowThreads), 0, stream, pdl, 1, x, ld, m, k, segs, oq, os)
-                   : launch(block_quant_rows_kernel<T, 4>, grid, dim3(kRowThreads), 0, stream, pdl, 1, x, ld, m, k, segs, oq, os);
+                   : launch(block_quant_rows_kernel<T, 2>, grid, dim3(kRowThreads), 0, stream, pdl, 1, x, ld, m, k, segs, oq, os);
     }
     const int64_t m_out = (m + 15) / 16 * 16;
     const dim3 grid(unsigned((m + kQBlock - 1) / kQBlock), unsigned((k + kQBlock - 1) / kQBlock), unsigned(batches));

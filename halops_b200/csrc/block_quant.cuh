@@ -94,12 +94,5 @@ __device__ __forceinline__ uint2 codes8(const uint4& v, const BlockScale& s) {
                       code2(two_floats<T>(v.z), s) | code2(two_floats<T>(v.w), s) << 16);
 }
 
-// Maximum over the 16 lanes that hold a block of 128 values.
-__device__ __forceinline__ uint32_t max16(uint32_t m) {
-#pragma unroll
-    for (int d = 1; d < 16; d *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
-    return m;
-}
-
 }  // namespace
 }  // namespace hq
