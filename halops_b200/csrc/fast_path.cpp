@@ -459,7 +459,7 @@ PyObject* moe_sort(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     if (ids == nullptr || ids->dim() != 2 || !ids->is_contiguous() || !small_int(a[1], &experts) || !small_int(a[2], &align) || !flag(a[3], &pdl)) {
         Py_RETURN_NONE;
     }
-    if ((ids->scalar_type() != at::kInt && ids->scalar_type() != at::kLong) || experts < 1 || experts > 1024 || align < 1 || align > 65536) {
+    if ((ids->scalar_type() != at::kInt && ids->scalar_type() != at::kLong) || experts < 1 || experts > 1024 || align < 1 || align > 4096) {
         Py_RETURN_NONE;
     }
     const int64_t n = ids->numel(), n_rows = (n + std::min<int64_t>(experts, n) * (align - 1)) / align * align;

@@ -514,7 +514,7 @@ extern "C" int hq_moe_sort(const void* ids, int ids_bytes, int64_t tokens, int64
     if (num_experts < 1) return fail(err, errlen, HQ_ERR_INVALID, "num_experts must be at least 1, got %lld", static_cast<long long>(num_experts));
     const int rc = hq::check_moe(tokens, topk, n_rows, num_experts, err, errlen);
     if (rc != HQ_OK) return rc;
-    if (align < 1 || align > 65536) return fail(err, errlen, HQ_ERR_INVALID, "align must be in [1, 65536], got %lld", static_cast<long long>(align));
+    if (align < 1 || align > 4096) return fail(err, errlen, HQ_ERR_INVALID, "align must be in [1, 4096], got %lld", static_cast<long long>(align));
     // any ids have to fit: what pads the runs of as many experts as there can be
     const int64_t n = tokens * topk, need = (n + (n < num_experts ? n : num_experts) * (align - 1)) / align * align;
     if (n_rows < need) {

@@ -47,7 +47,7 @@ def moe_sort(topk_ids: torch.Tensor, num_experts: int, align: int = 1, use_pdl: 
         topk_ids: [tokens, topk] contiguous CUDA tensor, int32 or int64.  Ids outside of [0, num_experts) are dropped (experts of another
             device: subtract the first one that is here).  A token may name an expert more than once.
         num_experts: experts here, at most 1024.
-        align: every run starts on a multiple of it; the rows that pad a run have no pair.
+        align: every run starts on a multiple of it, at most 4096; the rows that pad a run have no pair.
         use_pdl: launch with programmatic stream serialisation.
 
     Returns:
@@ -60,7 +60,7 @@ def moe_sort(topk_ids: torch.Tensor, num_experts: int, align: int = 1, use_pdl: 
     _check(topk_ids.dim() == 2, "topk_ids must be a 2D tensor of shape [tokens, topk]")
     _check(topk_ids.dtype in (torch.int32, torch.int64), "topk_ids must be int32 or int64")
     _check(1 <= num_experts <= MAX_EXPERTS, f"num_experts must be in [1, {MAX_EXPERTS}], got {num_experts}")
-    _check(1 <= align <= 65536, f"align must be in [1, 65536], got {align}")
+    _check(1 <= align <= 4096, f"align must be in [1, 4096], got {align}")
     _check(topk_ids.is_contiguous(), "topk_ids must be contiguous")
     _on_device(topk_ids.device, topk_ids=topk_ids)
     n = topk_ids.numel()
