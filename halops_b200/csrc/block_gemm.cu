@@ -341,6 +341,18 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     ptx::tc_fence_after();
     const uint32_t tmem = bars->tmem_base;
 
+    // A dense problem of few rows is bound by the weight's way from HBM: its first k-tiles are asked for into L2 while the preceding kernel
+    // finishes (a hint, so it may have been that kernel that wrote the weight).
+    if constexpr (!kGrouped) {
+        if (warp == kLoadWarp && p.pdl != 0 && p.tiles_m == 1) {
+            const int share = kSplit ? int(blockIdx.x) % p.split : 0, parts = kSplit ? p.split : 1;
+            const int n0 = (kSplit ? int(blockIdx.x) / parts : int(blockIdx.x)) * BN;
+            const int from = int(int64_t(p.k_tiles) * share / parts), to = int(int64_t(p.k_tiles) * (share + 1) / parts);
+            for (int kt = from; kt < min(to, from + 16); ++kt) {
+                if (ptx::elect_one()) ptx::tma_prefetch_2d(&tm_b, kt * kBlockK, n0);
+            }
+        }
+    }
     // nothing below may run before the preceding kernel's writes are visible
     ptx::pdl_wait();
     if constexpr (kGrouped) {
