@@ -93,7 +93,7 @@ struct BlockArgs {
     int experts;
     int box_rows;   // rows of `a` per copy
     int out_type;   // HQ_DTYPE_*
-    int out_align;  // 32, 16 or less: bytes that every row of the output starts on
+    int out_align;  // 32, 16, 4 or 2: bytes that every row of the output starts on
     int staged;     // 16-bit output that TMA can store
     int split;      // CTAs of a cluster that share a tile's k-tiles
     int wide_scales;  // both operands' scales are on 16 bytes
@@ -295,7 +295,9 @@ __device__ __forceinline__ void store_values(const float (&f)[kN], void* out, in
     }
 }
 
-template <int BN, bool kRowScales, bool kGrouped, bool kSplit>
+// kAnyRows: output rows on no 16 bytes.  (An instantiation of its own: as a branch it cost the 256-wide tile registers, 8192 x 8192 x 8192
+// 580 -> 615 us.)
+template <int BN, bool kRowScales, bool kGrouped, bool kSplit, bool kAnyRows>
 __global__ void __launch_bounds__((BlockCfg<BN, kRowScales>::kThreads), 1)
 block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_d,
                   const __grid_constant__ BlockArgs p) {
@@ -653,6 +655,59 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
                         }
                     }
                 }
+            } else if constexpr (kAnyRows) {
+                // Rows on no 16 bytes: 64 bytes of 32 rows at a time through the warp's slot, from where neighbouring lanes store neighbouring
+                // words.  (Each thread its row's values one by one: 5776 x 4740 x 5024 377 us, so 190.)
+                if (busy) {
+                    const uint32_t slot = epi_base + warp * (C::kEpiSlots * 2048);
+                    const bool f32 = p.out_type == HQ_DTYPE_FP32;
+                    const int rows = min(32, t.valid - quarter * 32);
+                    const int64_t row0 = t.row0 + quarter * 32;
+#pragma unroll
+                    for (int c = 0; c < C::kCols; c += 16) {
+                        const int col = t.n0 + part * C::kCols + c;
+                        if (col >= p.n) break;
+                        __syncwarp();
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t to = slot + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4);
+                            uint32_t w[4];
+                            if (f32) {
+#pragma unroll
+                                for (int l = 0; l < 4; ++l) w[l] = __float_as_uint(acc[c + j * 4 + l]);
+                            } else if (j < 2) {
+#pragma unroll
+                                for (int l = 0; l < 4; ++l) w[l] = pack16(acc[c + j * 8 + 2 * l], acc[c + j * 8 + 2 * l + 1], p.out_type);
+                            } else {
+                                continue;
+                            }
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                        }
+                        __syncwarp();
+                        // 16 values of a row: 16 lanes one each (float32, or rows on 2 bytes), or 8 lanes two each
+                        const int lanes = !f32 && p.out_align >= 4 ? 8 : 16, bytes = f32 || p.out_align >= 4 ? 4 : 2;
+                        const int at = lane % lanes * bytes, first = lane % lanes * (16 / lanes), left = p.n - col - first;
+                        for (int r = lane / lanes; r < rows; r += 32 / lanes) {
+                            const uint32_t from = slot + r * 64 + (((at >> 4) ^ ((r >> 1) & 3)) << 4) + (at & 15);
+                            const int64_t o = (row0 + r) * p.ldo + col + first;
+                            if (bytes == 4) {
+                                uint32_t w;
+                                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(from) : "memory");
+                                if (f32) {
+                                    if (left > 0) static_cast<uint32_t*>(p.out)[o] = w;
+                                } else if (left > 1) {
+                                    *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + o) = w;
+                                } else if (left > 0) {
+                                    static_cast<uint16_t*>(p.out)[o] = uint16_t(w);
+                                }
+                            } else {
+                                uint16_t w;
+                                asm volatile("ld.shared.b16 %0, [%1];" : "=h"(w) : "r"(from) : "memory");
+                                if (left > 0) static_cast<uint16_t*>(p.out)[o] = w;
+                            }
+                        }
+                    }
+                }
             } else if (p.staged != 0 && (kGrouped ? quarter * 32 + 32 <= t.valid : busy)) {
                 // 32 x 32 values at a time (rows and columns that are not there are dropped by the store; a run's last rows go the other way).
                 // 16-byte piece j of row r is at piece j ^ (r >> 1 & 3), the 64-byte swizzle of the tensor map.
@@ -757,11 +812,11 @@ struct BlockProblem {
     cudaStream_t stream;
 };
 
-template <int BN, bool kRowScales, bool kGrouped, bool kSplit>
+template <int BN, bool kRowScales, bool kGrouped, bool kSplit, bool kAnyRows = false>
 int launch_block_gemm(const BlockProblem& g, char* err, size_t errlen) {
     using C = BlockCfg<BN, kRowScales>;
     static SmemOptIn opt_in;
-    const auto kernel = block_gemm_kernel<BN, kRowScales, kGrouped, kSplit>;
+    const auto kernel = block_gemm_kernel<BN, kRowScales, kGrouped, kSplit, kAnyRows>;
     HQ_CUDA_TRY(opt_in.ensure(kernel, C::kSmemBytes));
     BlockArgs p = g.args;
     p.tiles_m = int((g.rows_a + kTileM - 1) / kTileM);
@@ -834,11 +889,12 @@ int launch_kind(const BlockProblem& g, char* err, size_t errlen) {
     if constexpr (kRowScales) {
         return launch_block_gemm<BN, true, false, false>(g, err, errlen);
     } else {
-        if (g.grouped) return launch_block_gemm<BN, false, true, false>(g, err, errlen);
+        const bool any = g.args.out_align < 16;
+        if (g.grouped) return any ? launch_block_gemm<BN, false, true, false, true>(g, err, errlen) : launch_block_gemm<BN, false, true, false>(g, err, errlen);
         if constexpr (BN <= 128) {
             if (g.args.split > 1) return launch_block_gemm<BN, false, false, true>(g, err, errlen);
         }
-        return launch_block_gemm<BN, false, false, false>(g, err, errlen);
+        return any ? launch_block_gemm<BN, false, false, false, true>(g, err, errlen) : launch_block_gemm<BN, false, false, false>(g, err, errlen);
     }
 }
 
@@ -886,7 +942,8 @@ int block_gemm(const void* a, const void* b, const float* sfa, const float* sfb,
     p.n_blocks = int((n + 127) / 128), p.experts = int(experts), p.out_type = out_type, p.pdl = use_pdl != 0;
     p.wide_scales = aligned(sfa, 16) && aligned(sfb, 16);
     const int64_t row_bytes = ldo * size;
-    p.out_align = aligned(out, 32) && row_bytes % 32 == 0 ? 32 : aligned(out, 16) && row_bytes % 16 == 0 ? 16 : size;
+    const auto starts = [&](int a) { return aligned(out, size_t(a)) && row_bytes % a == 0; };
+    p.out_align = starts(32) ? 32 : starts(16) ? 16 : starts(4) ? 4 : 2;
     // Rows of `a` per copy: all of a tile's, or about those of a run, so that short runs do not read their neighbours' rows.
     const int64_t mean = grouped ? (m + std::min(experts, m) - 1) / std::min(experts, m) : m;
     p.box_rows = 8;

@@ -124,7 +124,14 @@ __global__ void __launch_bounds__(kRowThreads) permute_block_quant_kernel(const 
     if (int(blockIdx.x) >= tokens) {
         const int e = int(blockIdx.x) - tokens;
         const BlockScale s = block_scale(0, true);
-        for (int r = min(offsets[e + 1], n_rows) - 1; r >= max(offsets[e], 0) && pairs[r] < 0; --r) {
+        // the first row without a pair, by halving
+        int first = max(offsets[e], 0);
+        const int end = min(offsets[e + 1], n_rows);
+        for (int n = end - first; n > 0;) {
+            const int half = n / 2;
+            if (pairs[first + half] >= 0) first += half + 1, n -= half + 1; else n = half;
+        }
+        for (int r = first; r < end; ++r) {
             if (c < k) {
                 *reinterpret_cast<uint4*>(q + int64_t(r) * k + c) = make_uint4(0, 0, 0, 0);
                 if ((threadIdx.x & 7) == 0) sf[int64_t(r) * kb + c / kQBlock] = s.scale;

@@ -14,6 +14,7 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <mutex>
 #include <type_traits>
 
@@ -186,6 +187,18 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const Id* __rest
     if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// The rows that pad expert e's run: [*first, *end), behind the rows with pairs.
+__device__ __forceinline__ void padding_of(const int* pairs, const int* offsets, int n_rows, int e, int* first, int* end) {
+    int lo = max(offsets[e], 0);
+    const int hi = min(offsets[e + 1], n_rows);
+    *end = hi;
+    for (int n = hi - lo; n > 0;) {  // the first row without a pair
+        const int half = n / 2;
+        if (pairs[lo + half] >= 0) lo += half + 1, n -= half + 1; else n = half;
+    }
+    *first = lo;
+}
+
 // ---------------------------------------------------------------------------- tokens to rows
 //
 // A CTA reads a piece of one token and writes it to each of the token's rows; the CTAs behind the tokens zero the rows that
@@ -202,7 +215,9 @@ __global__ void __launch_bounds__(kMoveThreads) moe_permute_kernel(const Unit* _
     const int c = blockIdx.y * (kMoveThreads * kPer) + threadIdx.x;
     if (int(blockIdx.x) >= tokens) {
         const int e = int(blockIdx.x) - tokens;
-        for (int r = min(offsets[e + 1], n_rows) - 1; r >= max(offsets[e], 0) && pairs[r] < 0; --r) {
+        int first, end;
+        padding_of(pairs, offsets, n_rows, e, &first, &end);
+        for (int r = first; r < end; ++r) {
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 if (c + i * kMoveThreads < units) out[int64_t(r) * units + c + i * kMoveThreads] = Unit{};
@@ -304,29 +319,52 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { re
 template <>
 __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-// kWide: pieces of 16 bytes (all rows start on 16 bytes), else single values.  A piece at `c` of a row of `h` values.
-template <typename T, bool kWide>
-struct Piece {
-    static constexpr int kN = kWide ? Floats<T>::kN : 1;
+// A piece of a row in one load: 16 bytes where all rows start on 16, pairs of 16-bit values where they start on 4, else single values.
+template <typename T, int kBytes>
+struct Piece;
+template <typename T>
+struct Piece<T, 16> {
+    static constexpr int kN = Floats<T>::kN;
     using Vec = typename Floats<T>::Vec;
     Vec v;
-    T one;
-    __device__ __forceinline__ void load(const T* p) {
-        if constexpr (kWide) v = __ldg(reinterpret_cast<const Vec*>(p)); else one = p[0];
-    }
+    __device__ __forceinline__ void load(const T* p) { v = __ldg(reinterpret_cast<const Vec*>(p)); }
+    __device__ __forceinline__ void get(float (&f)[kN]) const { Floats<T>::get(v, f); }
+    static __device__ __forceinline__ void store(T* p, const float (&f)[kN]) { *reinterpret_cast<Vec*>(p) = Floats<T>::put(f); }
+};
+template <typename T>
+struct Piece<T, 4> {
+    static constexpr int kN = 4 / int(sizeof(T));
+    uint32_t v;
+    __device__ __forceinline__ void load(const T* p) { v = __ldg(reinterpret_cast<const uint32_t*>(p)); }
     __device__ __forceinline__ void get(float (&f)[kN]) const {
-        if constexpr (kWide) Floats<T>::get(v, f); else f[0] = to_float(one);
+        T one[kN];
+        memcpy(one, &v, 4);
+#pragma unroll
+        for (int i = 0; i < kN; ++i) f[i] = to_float(one[i]);
     }
     static __device__ __forceinline__ void store(T* p, const float (&f)[kN]) {
-        if constexpr (kWide) *reinterpret_cast<Vec*>(p) = Floats<T>::put(f); else p[0] = from_float<T>(f[0]);
+        T one[kN];
+#pragma unroll
+        for (int i = 0; i < kN; ++i) one[i] = from_float<T>(f[i]);
+        uint32_t w;
+        memcpy(&w, one, 4);
+        *reinterpret_cast<uint32_t*>(p) = w;
     }
 };
+template <typename T>
+struct Piece<T, 2> {
+    static constexpr int kN = 1;
+    T one;
+    __device__ __forceinline__ void load(const T* p) { one = p[0]; }
+    __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = to_float(one); }
+    static __device__ __forceinline__ void store(T* p, const float (&f)[1]) { p[0] = from_float<T>(f[0]); }
+};
 
-template <typename T, bool kWide, int kPer>
+template <typename T, int kBytes, int kPer>
 __global__ void __launch_bounds__(kMoveThreads) moe_unpermute_kernel(const T* __restrict__ z, int64_t ld, int tokens, int h, int topk,
                                                                      const int* __restrict__ rows, int n_rows,
                                                                      const float* __restrict__ weights, T* __restrict__ y) {
-    using P = Piece<T, kWide>;
+    using P = Piece<T, kBytes>;
     constexpr int kSlots = 4;  // rows loaded before the first is added
     grid_wait();
     grid_launch_dependents();
@@ -380,13 +418,13 @@ __global__ void __launch_bounds__(kMoveThreads) moe_unpermute_kernel(const T* __
 // The gradients of the above: gz[row] = weight * gy[token], gw[pair] = <gy[token], z[row]>.  A group of kGroup threads has one pair
 // (a warp; a whole CTA where there are few pairs), with kAhead pieces of both rows in flight per thread; the pairs of a token are
 // neighbours, so that its gradient comes from HBM once.  The CTAs behind the pairs zero the rows that pad the runs.
-template <typename T, bool kWide, int kGroup>
+template <typename T, int kBytes, int kGroup>
 __global__ void __launch_bounds__(kMoveThreads) moe_unpermute_backward_kernel(
     const T* __restrict__ gy, int64_t ld_g, const T* __restrict__ z, int64_t ld_z, int pairs_n, int pair_ctas, int h, int topk,
     const int* __restrict__ rows, const int* __restrict__ pairs, const int* __restrict__ offsets, int n_rows,
     const float* __restrict__ weights, T* __restrict__ gz, float* __restrict__ gw) {
-    using P = Piece<T, kWide>;
-    constexpr int kAhead = 4, kStep = kGroup * P::kN;
+    using P = Piece<T, kBytes>;
+    constexpr int kAhead = kBytes == 16 ? 4 : 8, kStep = kGroup * P::kN;
     __shared__ float parts[kMoveThreads / 32];
     grid_wait();
     grid_launch_dependents();
@@ -395,7 +433,9 @@ __global__ void __launch_bounds__(kMoveThreads) moe_unpermute_backward_kernel(
         float zero[P::kN];
 #pragma unroll
         for (int i = 0; i < P::kN; ++i) zero[i] = 0.0f;
-        for (int r = min(offsets[e + 1], n_rows) - 1; r >= max(offsets[e], 0) && pairs[r] < 0; --r) {
+        int first, end;
+        padding_of(pairs, offsets, n_rows, e, &first, &end);
+        for (int r = first; r < end; ++r) {
             for (int c = threadIdx.x * P::kN; c < h; c += kMoveThreads * P::kN) P::store(gz + int64_t(r) * h + c, zero);
         }
         return;
@@ -483,7 +523,7 @@ cudaError_t launch_sort(const void* ids, int pairs_n, int experts, int align, in
 template <typename Unit>
 cudaError_t launch_permute(const void* x, int64_t ld_bytes, int64_t tokens, int64_t row_bytes, int topk, const int* rows, const int* pairs,
                            const int* offsets, int64_t experts, int n_rows, void* out, bool pdl, cudaStream_t stream) {
-    constexpr int kPer = sizeof(Unit) == 16 ? 2 : 4;
+    constexpr int kPer = sizeof(Unit) == 16 ? 2 : sizeof(Unit) == 4 ? 4 : 8;
     const int units = int(row_bytes / int64_t(sizeof(Unit)));
     const dim3 grid(unsigned(tokens + experts), unsigned((units + kMoveThreads * kPer - 1) / (kMoveThreads * kPer)));
     return launch(moe_permute_kernel<Unit, kPer>, grid, dim3(kMoveThreads), 0, stream, pdl, 1, static_cast<const Unit*>(x),
@@ -575,11 +615,13 @@ extern "C" int hq_moe_unpermute(const void* input, int64_t ld_elems, int dtype, 
     }
     const hq::DeviceGuard guard(device);
     if (!guard.ok()) return fail(err, errlen, HQ_ERR_CUDA, "cannot select CUDA device %d", device);
-    const bool wide = hq::aligned(input, 16) && hq::aligned(output, 16) && ld_elems * size % 16 == 0 && h * size % 16 == 0;
-    // two pieces a thread where rows fill them and there are tokens for all SMs: more bytes in flight per CTA
-    const int64_t one = hq::kMoveThreads * int64_t(wide ? 16 / size : 1);
-    const bool two = wide && h >= 2 * one && tokens >= 1024;
-    const int64_t per = two ? 2 * one : one;
+    const auto fits = [&](int a) { return hq::aligned(input, a) && hq::aligned(output, a) && ld_elems * size % a == 0 && h * size % a == 0; };
+    const int bytes = fits(16) ? 16 : fits(4) ? 4 : 2;
+    // several pieces a thread where rows fill them and there are tokens for all SMs: more bytes in flight per CTA
+    const int64_t one = hq::kMoveThreads * int64_t(std::max(1, bytes / size));
+    const int pieces = bytes == 16 ? 2 : 4;
+    const bool many = h >= pieces * one && tokens >= 1024;
+    const int64_t per = many ? pieces * one : one;
     const dim3 grid(unsigned(tokens), unsigned((h + per - 1) / per));
     const auto go = [&](auto kernel, auto* z) {
         using T = std::remove_const_t<std::remove_pointer_t<decltype(z)>>;
@@ -588,9 +630,11 @@ extern "C" int hq_moe_unpermute(const void* input, int64_t ld_elems, int dtype, 
     };
     const auto typed = [&](auto* z) {
         using T = std::remove_const_t<std::remove_pointer_t<decltype(z)>>;
-        return !wide ? go(hq::moe_unpermute_kernel<T, false, 1>, z)
-               : two ? go(hq::moe_unpermute_kernel<T, true, 2>, z)
-                     : go(hq::moe_unpermute_kernel<T, true, 1>, z);
+        if (bytes == 16) return many ? go(hq::moe_unpermute_kernel<T, 16, 2>, z) : go(hq::moe_unpermute_kernel<T, 16, 1>, z);
+        if constexpr (sizeof(T) == 2) {
+            if (bytes == 2) return many ? go(hq::moe_unpermute_kernel<T, 2, 4>, z) : go(hq::moe_unpermute_kernel<T, 2, 1>, z);
+        }
+        return many ? go(hq::moe_unpermute_kernel<T, 4, 4>, z) : go(hq::moe_unpermute_kernel<T, 4, 1>, z);
     };
     HQ_CUDA_TRY(dtype == HQ_DTYPE_BF16   ? typed(static_cast<const __nv_bfloat16*>(input))
                 : dtype == HQ_DTYPE_FP16 ? typed(static_cast<const __half*>(input))
@@ -615,8 +659,11 @@ extern "C" int hq_moe_unpermute_backward(const void* grad_output, int64_t ld_gra
     }
     const hq::DeviceGuard guard(device);
     if (!guard.ok()) return fail(err, errlen, HQ_ERR_CUDA, "cannot select CUDA device %d", device);
-    const bool wide = hq::aligned(grad_output, 16) && hq::aligned(grad_input, 16) && hq::aligned(input, 16) && ld_grad * size % 16 == 0 &&
-                      ld_input * size % 16 == 0 && h * size % 16 == 0;
+    const auto fits = [&](int a) {
+        return hq::aligned(grad_output, a) && hq::aligned(grad_input, a) && hq::aligned(input, a) && ld_grad * size % a == 0 &&
+               ld_input * size % a == 0 && h * size % a == 0;
+    };
+    const int bytes = fits(16) ? 16 : fits(4) ? 4 : 2;
     // a warp per pair once they fill the SMs (148 of 16 CTAs' warps), else a CTA
     const int64_t n = tokens * topk;
     const bool warps = n >= 148 * 16;
@@ -630,8 +677,12 @@ extern "C" int hq_moe_unpermute_backward(const void* grad_output, int64_t ld_gra
     };
     const auto typed = [&](auto* g) {
         using T = std::remove_const_t<std::remove_pointer_t<decltype(g)>>;
-        return wide ? (warps ? go(hq::moe_unpermute_backward_kernel<T, true, 32>, g) : go(hq::moe_unpermute_backward_kernel<T, true, hq::kMoveThreads>, g))
-                    : (warps ? go(hq::moe_unpermute_backward_kernel<T, false, 32>, g) : go(hq::moe_unpermute_backward_kernel<T, false, hq::kMoveThreads>, g));
+        constexpr int kAll = hq::kMoveThreads;
+        if (bytes == 16) return warps ? go(hq::moe_unpermute_backward_kernel<T, 16, 32>, g) : go(hq::moe_unpermute_backward_kernel<T, 16, kAll>, g);
+        if constexpr (sizeof(T) == 2) {
+            if (bytes == 2) return warps ? go(hq::moe_unpermute_backward_kernel<T, 2, 32>, g) : go(hq::moe_unpermute_backward_kernel<T, 2, kAll>, g);
+        }
+        return warps ? go(hq::moe_unpermute_backward_kernel<T, 4, 32>, g) : go(hq::moe_unpermute_backward_kernel<T, 4, kAll>, g);
     };
     HQ_CUDA_TRY(dtype == HQ_DTYPE_BF16   ? typed(static_cast<const __nv_bfloat16*>(grad_output))
                 : dtype == HQ_DTYPE_FP16 ? typed(static_cast<const __half*>(grad_output))
