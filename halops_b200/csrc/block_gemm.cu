@@ -30,9 +30,6 @@ namespace {
 
 constexpr int kTileM = 128;
 constexpr int kBlockK = 128;  // values, and bytes, of a k-tile row
-constexpr int kParts = 2;  // groups of four warps that share a tile's columns
-constexpr int kPromoWarps = 4 * kParts;
-constexpr int kLoadWarp = kPromoWarps, kScaleWarp = kPromoWarps + 1, kMmaWarp = kPromoWarps + 2;  // and kMmaWarp + 1
 constexpr int kMaxExperts = 1024;
 constexpr int kSmemBudget = 232448;
 constexpr int kGroupK = 4;      // k-tiles whose scales are brought together
@@ -51,10 +48,13 @@ struct BlockBars {
 
 template <int BN, bool kRowScales>
 struct BlockCfg {
+    static constexpr int kParts = BN == 192 ? 3 : 2;  // groups of four warps that share a tile's columns
+    static constexpr int kPromoWarps = 4 * kParts;
+    static constexpr int kLoadWarp = kPromoWarps, kScaleWarp = kPromoWarps + 1, kMmaWarp = kPromoWarps + 2;  // and kMmaWarp + 1
     // k-tiles of a step, which share a stage and a set of buffers: what a step's waits and signals cost (400 to 500 cycles from role to
     // role) is more than a narrow tile's k-tile has to do, 16 x 4096 x 7168 on 64 columns takes 11.8 us in steps of two and 13.1 of one,
     // 8192 x 8192 x 8192 on 128 columns 579 and 615
-    static constexpr int kStep = BN == 256 ? 1 : 2;
+    static constexpr int kStep = BN > 128 ? 1 : 2;
     static constexpr int kABytes = kTileM * kBlockK;  // per k-tile
     static constexpr int kBBytes = BN * kBlockK;
     static constexpr int kStageBytes = kStep * (kABytes + kBBytes);
@@ -65,21 +65,21 @@ struct BlockCfg {
     static constexpr int kScales = kRowScales ? kTileM + BN : kTileM * kWeightBlocks;
     static constexpr int kScaleBytes = kScaleSlots * kGroupK * kScales * 4;
     // a warp's finished 32 x 32 values on their way to a TMA store; all of a 256-wide tile's at a time
-    static constexpr int kEpiSlots = kRowScales ? 0 : BN == 256 ? 4 : 1;
+    static constexpr int kEpiSlots = kRowScales ? 0 : BN == 256 ? 4 : BN == 192 ? 2 : 1;
     static constexpr int kEpiBytes = kPromoWarps * kEpiSlots * 2048;
     static constexpr int kExtra = kBarBytes + kTableBytes + kScaleBytes + kEpiBytes + 1024;
     static constexpr int kFit = (kSmemBudget - kExtra) / kStageBytes;
     static constexpr int kStages = kFit;
     static constexpr int kSmemBytes = kStages * kStageBytes + kExtra;
     static constexpr int kBufs = 2;  // of kStep accumulators each
-    static constexpr int kTmemCols = kBufs * kStep * BN;
+    static constexpr int kTmemCols = BN == 192 ? 512 : kBufs * kStep * BN;  // (a power of two)
     static constexpr int kCols = BN / kParts;  // columns of a promotion warp
-    static constexpr int kLd = BN == 64 ? 32 : 16;  // of which one load brings
+    static constexpr int kLd = BN == 64 || BN == 192 ? 32 : 16;  // of which one load brings
     static constexpr int kThreads = (kPromoWarps + 4) * 32;
     // BN = 256: 128 accumulators a thread; the third warpgroup gives registers to the other two (168 * 384 = 208 * 256 + 88 * 128)
     static constexpr bool kRegSplit = BN == 256;
     static_assert(sizeof(BlockBars) <= kBarBytes && kStages >= 3 && kStages <= 8 && kTmemCols <= 512, "budgets");
-    static_assert(kTileM * (BN + 4) * 4 <= kStages * kStageBytes, "split-K partial sums fit into the ring");
+    static_assert(BN > 128 || kTileM * (BN + 4) * 4 <= kStages * kStageBytes, "split-K partial sums fit into the ring");
 };
 
 struct BlockArgs {
@@ -322,11 +322,11 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         }
         for (int s = 0; s < C::kBufs; ++s) {
             ptx::mbar_init(ptx::smem_u32(&bars->acc_full[s]), C::kStep);
-            ptx::mbar_init(ptx::smem_u32(&bars->acc_empty[s]), kPromoWarps);
+            ptx::mbar_init(ptx::smem_u32(&bars->acc_empty[s]), C::kPromoWarps);
         }
         for (int s = 0; s < kScaleSlots; ++s) {
             ptx::mbar_init(ptx::smem_u32(&bars->sf_full[s]), 1);
-            ptx::mbar_init(ptx::smem_u32(&bars->sf_empty[s]), kPromoWarps);
+            ptx::mbar_init(ptx::smem_u32(&bars->sf_empty[s]), C::kPromoWarps);
         }
         bars->abort = 0;
         ptx::fence_mbar_init();
@@ -334,7 +334,7 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         ptx::prefetch_tmap(&tm_b);
         if (p.staged != 0) ptx::prefetch_tmap(&tm_d);
     }
-    if (warp == kMmaWarp) {
+    if (warp == C::kMmaWarp) {
         ptx::tmem_alloc<1>(ptx::smem_u32(&bars->tmem_base), C::kTmemCols);
         ptx::tmem_relinquish<1>();
     }
@@ -346,7 +346,7 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     // A dense problem of few rows is bound by the weight's way from HBM: its first k-tiles are asked for into L2 while the preceding kernel
     // finishes (a hint, so it may have been that kernel that wrote the weight).
     if constexpr (!kGrouped) {
-        if (warp == kLoadWarp && p.pdl != 0 && p.tiles_m == 1) {
+        if (warp == C::kLoadWarp && p.pdl != 0 && p.tiles_m == 1) {
             const int share = kSplit ? int(blockIdx.x) % p.split : 0, parts = kSplit ? p.split : 1;
             const int n0 = (kSplit ? int(blockIdx.x) / parts : int(blockIdx.x)) * BN;
             const int from = int(int64_t(p.k_tiles) * share / parts), to = int(int64_t(p.k_tiles) * (share + 1) / parts);
@@ -398,9 +398,9 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     const int k_begin = kSplit ? int(int64_t(steps) * rank / p.split) * C::kStep : 0;
     const int k_end = kSplit ? min(int(int64_t(steps) * (rank + 1) / p.split) * C::kStep, p.k_tiles) : p.k_tiles;
 
-    if (warp >= kPromoWarps) {
+    if (warp >= C::kPromoWarps) {
     if constexpr (C::kRegSplit) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == kLoadWarp) {
+    if (warp == C::kLoadWarp) {
         // ------------------------------------------------------------ TMA producer
         uint32_t it = 0;
         bool ok = true;
@@ -440,13 +440,13 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         for (uint32_t d = it > uint32_t(C::kStages) ? it - C::kStages : 0u; ok && d < it; ++d) {
             ok = wait_bar<C::kRegSplit>(ptx::smem_u32(&bars->empty[d % C::kStages]), (d / C::kStages) & 1u, abort, kStatusProducer);
         }
-    } else if (warp >= kMmaWarp && warp < kMmaWarp + C::kStep) {
+    } else if (warp >= C::kMmaWarp && warp < C::kMmaWarp + C::kStep) {
         // ------------------------------------------------------------ MMA issuers
         // One for each k-tile of a step.  Every k-tile has a buffer of its own, so nothing has to be kept in order between them.  (Two that took
         // turns at the steps would skip phases of the stages' barriers, and a wait for the next but one is over before it began.)
         // float32 sums, e4m3 operands, both K-major; N >> 3, M >> 4
         constexpr uint32_t idesc = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(kTileM >> 4) << 24);
-        const uint32_t u = warp - kMmaWarp;
+        const uint32_t u = warp - C::kMmaWarp;
         const uint64_t adesc0 = ptx::smem_desc(a_base, 16, 1024, 2), bdesc0 = ptx::smem_desc(b_base, 16, 1024, 2);
         uint32_t it = 0;
         bool ok = true;
@@ -472,7 +472,7 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
                 }
             }
         }
-    } else if (warp == kScaleWarp) {
+    } else if (warp == C::kScaleWarp) {
         // ------------------------------------------------------------ scales
         // A group's are in registers before its slot is free.  A lane has every 32nd row; four neighbouring k-tiles are one load where
         // they lie on 16 bytes.
@@ -564,7 +564,7 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
 #pragma unroll
                             for (int q = 0; q < 4; ++q) s[u][q] = from[(i + u) * C::kScales + quarter * 32 + q * 8 + lane / 4];
                         } else {
-                            s[u][0] = from[(i + u) * C::kScales + (C::kWeightBlocks == 2 ? part * 2 / kParts * kTileM : 0) + row];
+                            s[u][0] = from[(i + u) * C::kScales + (C::kWeightBlocks == 2 ? (t.n0 % 128 + part * C::kCols) / 128 * kTileM : 0) + row];
                         }
                     }
                     ok = wait_bar<C::kRegSplit>(ptx::smem_u32(&bars->acc_full[buf]), (it / C::kBufs) & 1u, abort, kStatusEpilogue);
@@ -751,21 +751,21 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
         }
     }
 
-    if (!kSplit && !kRowScales && warp < kPromoWarps && lane == 0) ptx::bulk_wait<0>();
+    if (!kSplit && !kRowScales && warp < C::kPromoWarps && lane == 0) ptx::bulk_wait<0>();
     __syncwarp();
 
     if constexpr (kSplit) {
         // One tile per cluster: every CTA adds up its share of the tile over the CTAs, in their order.
         __syncwarp();
         ptx::cluster_sync();
-        if (warp < kPromoWarps) {
+        if (warp < C::kPromoWarps) {
             BlockWalk<BN, kGrouped> walk(p, tables, first, step);
             BlockTile t;
             if (walk.next(t)) {
                 constexpr int kVecs = BN / 4;
                 const int total = t.valid * kVecs;
                 const int end = int(int64_t(total) * (rank + 1) / p.split);
-                for (int i = int(int64_t(total) * rank / p.split) + threadIdx.x; i < end; i += kPromoWarps * 32) {
+                for (int i = int(int64_t(total) * rank / p.split) + threadIdx.x; i < end; i += C::kPromoWarps * 32) {
                     const int r = i / kVecs, c = (i - r * kVecs) * 4;
                     const uint32_t addr = a_base + (r * (BN + 4) + c) * 4;
                     float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -794,7 +794,7 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     __syncthreads();
     // no CTA leaves while another reads its sums
     if constexpr (kSplit) ptx::cluster_sync();
-    if (warp == kMmaWarp) {
+    if (warp == C::kMmaWarp) {
         ptx::tc_fence_after();
         ptx::tmem_dealloc<1>(tmem, C::kTmemCols);
     }
@@ -952,6 +952,7 @@ int block_gemm(const void* a, const void* b, const float* sfa, const float* sfb,
     p.split = c.split;
     if (g.row_scales) return c.bn == 128 ? launch_kind<128, true>(g, err, errlen) : launch_kind<64, true>(g, err, errlen);
     return c.bn == 256   ? launch_kind<256, false>(g, err, errlen)
+           : c.bn == 192 ? launch_kind<192, false>(g, err, errlen)
            : c.bn == 128 ? launch_kind<128, false>(g, err, errlen)
                          : launch_kind<64, false>(g, err, errlen);
 }
