@@ -859,7 +859,7 @@ BlockChoice choose(const BlockProblem& g) {
         int bn;
         double alone, full, tile;
     };
-    constexpr Cost kCosts[] = {{128, 0.20, 0.30, 1.0}, {64, 0.157, 0.21, 0.7}, {256, 0.42, 0.53, 1.6}};  // (in order of preference where the floor decides)
+    constexpr Cost kCosts[] = {{128, 0.20, 0.30, 1.0}, {64, 0.157, 0.21, 0.7}, {192, 0.30, 0.42, 1.2}, {256, 0.42, 0.53, 1.6}};  // (in order of preference where the floor decides)
     const int k_tiles = g.args.k_tiles;
     const int64_t runs = std::min(g.experts, g.rows_a);  // with rows
     const int64_t mean = (g.rows_a + runs - 1) / runs;
@@ -869,11 +869,11 @@ BlockChoice choose(const BlockProblem& g) {
     BlockChoice best = {128, 1};
     double least = 1e30;
     for (const Cost& c : kCosts) {
-        if (g.row_scales && c.bn == 256) continue;
+        if (g.row_scales && c.bn > 128) continue;
         const int64_t tiles = row_tiles * ((g.n + c.bn - 1) / c.bn);
         for (int split = 1; split <= 8; split *= 2) {
             // (clusters of 8 do not fill every group of SMs)
-            if (split > 1 && (g.grouped || g.row_scales || c.bn == 256 || tiles * split > (split == 8 ? g.sms * 6 / 7 : g.sms) || k_tiles < 4 * split)) break;
+            if (split > 1 && (g.grouped || g.row_scales || c.bn > 128 || tiles * split > (split == 8 ? g.sms * 6 / 7 : g.sms) || k_tiles < 4 * split)) break;
             const int64_t ctas = tiles * split, waves = (ctas + g.sms - 1) / g.sms;
             const double busy = double(std::min<int64_t>(ctas, g.sms)) / g.sms;
             const double step = c.alone + (c.full - c.alone) * busy;
