@@ -6,12 +6,21 @@
 // so a float32 scale cannot ride along with the MMA: the products of one block of 128 are summed in tensor memory (four MMAs,
 // K = 32 each), and the sums then leave for registers, where they are scaled and added up in float32.
 //
-// Per CTA (one per SM, persistent over output tiles of 128 x BN):
-//   warps 0-7  promotion: tcgen05.ld of a block's sums, accumulators += scale * sums (two columns an instruction); after the last
-//              block the accumulators are rounded once and stored.  A thread has one row and half of the tile's columns.
-//   warp 8     TMA producer: A and B tiles (128-byte swizzle) into a ring of stages
-//   warps 10, 11  issue the MMAs of a step (BN = 256: one block; else two, one each) into the next of 2 sets of buffers in tensor memory
-//   warp 9     brings the scales of four blocks at a time into shared memory, multiplied where a row has one factor per block
+// Per CTA (one per SM, persistent over output tiles of 128 x BN, BN = 64, 128, 192 or 256):
+//   8 warps (BN = 192: 12)  promotion: tcgen05.ld of a block's sums, accumulators += scale * sums (two columns an instruction); after the
+//               last block the accumulators are rounded once and stored.  A thread has one row and a half (a third) of the tile's columns.
+//   1 warp      TMA producer: A and B tiles (128-byte swizzle) into a ring of stages
+//   1 warp      brings the scales of four blocks at a time into shared memory, multiplied where a row has one factor per block (loaded by the
+//               threads that use them, a float of a row each, they took a sixth of the time: 8192 x 8192 x 8192 625 us, 537 without)
+//   1 or 2 warps  issue the MMAs of a step (BN > 128: one block; else two, one each) into the next of 2 sets of buffers in tensor memory
+//
+// What bounds it.  A step is a round between the roles: MMAs (512 cycles on 256 columns), commit and wake-up (100), loads and products of
+// the promotion (about 70 cycles for each 16 columns of its two warps a scheduler, which wait for the loads together: 560), the signal back
+// (100 to 200); with two sets of buffers half of that is hidden, 850 to 870 cycles a block.  The tensor pipe is busy for half of
+// the time (ncu: 52 % on 4096 x 7168 x 2048), L2 for a third.  Large problems run at the power cap besides: 8192 x 8192 x 8192 takes 545 to
+// 605 us at 1.38 GHz and 990 W (the MXFP8 kernel, whose scales cost no such round, 432 at 1.17).  Measured and left: 16 promotion warps on 256
+// columns (registers spill; 595 us against 540), double-buffered loads (648), half of B's bytes, as a CTA pair would load (518 without what
+// a pair's remote signals would add).
 //
 // Every mbarrier wait is bounded, as in the other GEMM kernels: a role that waits longer than kTimeoutNs records a code in the
 // status word, raises the CTA's abort flag and all roles leave through the common teardown.
@@ -399,139 +408,139 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
     const int k_end = kSplit ? min(int(int64_t(steps) * (rank + 1) / p.split) * C::kStep, p.k_tiles) : p.k_tiles;
 
     if (warp >= C::kPromoWarps) {
-    if constexpr (C::kRegSplit) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == C::kLoadWarp) {
-        // ------------------------------------------------------------ TMA producer
-        uint32_t it = 0;
-        bool ok = true;
-        BlockWalk<BN, kGrouped> walk(p, tables, first, step);
-        BlockTile t;
-        while (ok && walk.next(t)) {
-            const int boxes = (t.valid + p.box_rows - 1) / p.box_rows;
-            const int b_row = t.expert * p.n + t.n0;
-            const uint32_t bytes = C::kStep * uint32_t(boxes * p.box_rows * kBlockK + C::kBBytes);
-            for (int kt = k_begin; kt < k_end; kt += C::kStep, ++it) {
-                const uint32_t s = it % C::kStages;
-                ok = wait_bar<C::kRegSplit>(ptx::smem_u32(&bars->empty[s]), ((it / C::kStages) & 1u) ^ 1u, abort, kStatusProducer);
-                if (!ok) break;
-                const uint32_t full = ptx::smem_u32(&bars->full[s]);
-                const uint32_t a_to = a_base + s * (C::kStep * C::kABytes), b_to = b_base + s * (C::kStep * C::kBBytes);
-                if (ptx::elect_one()) {
-                    ptx::mbar_arrive_expect_tx(full, bytes);
-#pragma unroll
-                    for (int u = 0; u < C::kStep; ++u) {
-                        ptx::tma_load_2d(b_to + u * C::kBBytes, &tm_b, (kt + u) * kBlockK, b_row, full);
-                        ptx::tma_load_2d(a_to + u * C::kABytes, &tm_a, (kt + u) * kBlockK, t.row0, full);
-                    }
-                }
-                for (int b = 1; b < boxes; ++b) {
-                    const int skip = b * p.box_rows;
+        if constexpr (C::kRegSplit) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == C::kLoadWarp) {
+            // ------------------------------------------------------------ TMA producer
+            uint32_t it = 0;
+            bool ok = true;
+            BlockWalk<BN, kGrouped> walk(p, tables, first, step);
+            BlockTile t;
+            while (ok && walk.next(t)) {
+                const int boxes = (t.valid + p.box_rows - 1) / p.box_rows;
+                const int b_row = t.expert * p.n + t.n0;
+                const uint32_t bytes = C::kStep * uint32_t(boxes * p.box_rows * kBlockK + C::kBBytes);
+                for (int kt = k_begin; kt < k_end; kt += C::kStep, ++it) {
+                    const uint32_t s = it % C::kStages;
+                    ok = wait_bar<C::kRegSplit>(ptx::smem_u32(&bars->empty[s]), ((it / C::kStages) & 1u) ^ 1u, abort, kStatusProducer);
+                    if (!ok) break;
+                    const uint32_t full = ptx::smem_u32(&bars->full[s]);
+                    const uint32_t a_to = a_base + s * (C::kStep * C::kABytes), b_to = b_base + s * (C::kStep * C::kBBytes);
                     if (ptx::elect_one()) {
+                        ptx::mbar_arrive_expect_tx(full, bytes);
 #pragma unroll
                         for (int u = 0; u < C::kStep; ++u) {
-                            ptx::tma_load_2d(a_to + u * C::kABytes + skip * kBlockK, &tm_a, (kt + u) * kBlockK, t.row0 + skip, full);
+                            ptx::tma_load_2d(b_to + u * C::kBBytes, &tm_b, (kt + u) * kBlockK, b_row, full);
+                            ptx::tma_load_2d(a_to + u * C::kABytes, &tm_a, (kt + u) * kBlockK, t.row0, full);
+                        }
+                    }
+                    for (int b = 1; b < boxes; ++b) {
+                        const int skip = b * p.box_rows;
+                        if (ptx::elect_one()) {
+#pragma unroll
+                            for (int u = 0; u < C::kStep; ++u) {
+                                ptx::tma_load_2d(a_to + u * C::kABytes + skip * kBlockK, &tm_a, (kt + u) * kBlockK, t.row0 + skip, full);
+                            }
                         }
                     }
                 }
             }
-        }
-        ptx::pdl_launch_dependents();
-        // the releases of the last stages arrive in this CTA's shared memory: it is not left before they have
-        for (uint32_t d = it > uint32_t(C::kStages) ? it - C::kStages : 0u; ok && d < it; ++d) {
-            ok = wait_bar<C::kRegSplit>(ptx::smem_u32(&bars->empty[d % C::kStages]), (d / C::kStages) & 1u, abort, kStatusProducer);
-        }
-    } else if (warp >= C::kMmaWarp && warp < C::kMmaWarp + C::kStep) {
-        // ------------------------------------------------------------ MMA issuers
-        // One for each k-tile of a step.  Every k-tile has a buffer of its own, so nothing has to be kept in order between them.  (Two that took
-        // turns at the steps would skip phases of the stages' barriers, and a wait for the next but one is over before it began.)
-        // float32 sums, e4m3 operands, both K-major; N >> 3, M >> 4
-        constexpr uint32_t idesc = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(kTileM >> 4) << 24);
-        const uint32_t u = warp - C::kMmaWarp;
-        const uint64_t adesc0 = ptx::smem_desc(a_base, 16, 1024, 2), bdesc0 = ptx::smem_desc(b_base, 16, 1024, 2);
-        uint32_t it = 0;
-        bool ok = true;
-        BlockWalk<BN, kGrouped> walk(p, tables, first, step);
-        BlockTile t;
-        while (ok && walk.next(t)) {
-            for (int kt = k_begin; kt < k_end; kt += C::kStep, ++it) {
-                const uint32_t s = it % C::kStages, buf = it % C::kBufs;
-                ok = wait_bars<C::kRegSplit>(ptx::smem_u32(&bars->full[s]), (it / C::kStages) & 1u, true, ptx::smem_u32(&bars->acc_empty[buf]),
-                               ((it / C::kBufs) & 1u) ^ 1u, abort, kStatusMma);
-                if (!ok) break;
-                ptx::tc_fence_after();
-                // (addresses are in the descriptors' low bits, in units of 16 bytes; K = 32 bytes is a step of 2 inside of the swizzle atom)
-                const uint64_t adesc = adesc0 + (s * C::kStep + u) * (C::kABytes >> 4), bdesc = bdesc0 + (s * C::kStep + u) * (C::kBBytes >> 4);
-                const uint32_t d = tmem + (buf * C::kStep + u) * BN;
-                if (ptx::elect_one()) {
-                    mma_e4m3(d, adesc, bdesc, idesc, 0u);
-                    mma_e4m3(d, adesc + 2, bdesc + 2, idesc, 1u);
-                    mma_e4m3(d, adesc + 4, bdesc + 4, idesc, 1u);
-                    mma_e4m3(d, adesc + 6, bdesc + 6, idesc, 1u);
-                    ptx::tc_commit(ptx::smem_u32(&bars->acc_full[buf]));
-                    ptx::tc_commit(ptx::smem_u32(&bars->empty[s]));
+            ptx::pdl_launch_dependents();
+            // the releases of the last stages arrive in this CTA's shared memory: it is not left before they have
+            for (uint32_t d = it > uint32_t(C::kStages) ? it - C::kStages : 0u; ok && d < it; ++d) {
+                ok = wait_bar<C::kRegSplit>(ptx::smem_u32(&bars->empty[d % C::kStages]), (d / C::kStages) & 1u, abort, kStatusProducer);
+            }
+        } else if (warp >= C::kMmaWarp && warp < C::kMmaWarp + C::kStep) {
+            // ------------------------------------------------------------ MMA issuers
+            // One for each k-tile of a step.  Every k-tile has a buffer of its own, so nothing has to be kept in order between them.  (Two that took
+            // turns at the steps would skip phases of the stages' barriers, and a wait for the next but one is over before it began.)
+            // float32 sums, e4m3 operands, both K-major; N >> 3, M >> 4
+            constexpr uint32_t idesc = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(kTileM >> 4) << 24);
+            const uint32_t u = warp - C::kMmaWarp;
+            const uint64_t adesc0 = ptx::smem_desc(a_base, 16, 1024, 2), bdesc0 = ptx::smem_desc(b_base, 16, 1024, 2);
+            uint32_t it = 0;
+            bool ok = true;
+            BlockWalk<BN, kGrouped> walk(p, tables, first, step);
+            BlockTile t;
+            while (ok && walk.next(t)) {
+                for (int kt = k_begin; kt < k_end; kt += C::kStep, ++it) {
+                    const uint32_t s = it % C::kStages, buf = it % C::kBufs;
+                    ok = wait_bars<C::kRegSplit>(ptx::smem_u32(&bars->full[s]), (it / C::kStages) & 1u, true, ptx::smem_u32(&bars->acc_empty[buf]),
+                                   ((it / C::kBufs) & 1u) ^ 1u, abort, kStatusMma);
+                    if (!ok) break;
+                    ptx::tc_fence_after();
+                    // (addresses are in the descriptors' low bits, in units of 16 bytes; K = 32 bytes is a step of 2 inside of the swizzle atom)
+                    const uint64_t adesc = adesc0 + (s * C::kStep + u) * (C::kABytes >> 4), bdesc = bdesc0 + (s * C::kStep + u) * (C::kBBytes >> 4);
+                    const uint32_t d = tmem + (buf * C::kStep + u) * BN;
+                    if (ptx::elect_one()) {
+                        mma_e4m3(d, adesc, bdesc, idesc, 0u);
+                        mma_e4m3(d, adesc + 2, bdesc + 2, idesc, 1u);
+                        mma_e4m3(d, adesc + 4, bdesc + 4, idesc, 1u);
+                        mma_e4m3(d, adesc + 6, bdesc + 6, idesc, 1u);
+                        ptx::tc_commit(ptx::smem_u32(&bars->acc_full[buf]));
+                        ptx::tc_commit(ptx::smem_u32(&bars->empty[s]));
+                    }
                 }
             }
-        }
-    } else if (warp == C::kScaleWarp) {
-        // ------------------------------------------------------------ scales
-        // A group's are in registers before its slot is free.  A lane has every 32nd row; four neighbouring k-tiles are one load where
-        // they lie on 16 bytes.
-        constexpr int kRowsA = kTileM / 32, kRowsB = kRowScales ? BN / 32 : 1;
-        const bool wide = p.k_tiles % 4 == 0 && p.wide_scales != 0;
-        const auto load4 = [&](const float* q, int k0, float (&v)[kGroupK]) {
-            if (wide && k0 % 4 == 0 && k0 + kGroupK <= k_end) {
-                const float4 f = __ldg(reinterpret_cast<const float4*>(q + k0));
-                v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-            } else {
-#pragma unroll
-                for (int i = 0; i < kGroupK; ++i) v[i] = k0 + i < k_end ? __ldg(q + k0 + i) : 0.0f;
-            }
-        };
-        uint32_t group = 0;
-        bool ok = true;
-        BlockWalk<BN, kGrouped> walk(p, tables, first, step);
-        BlockTile t;
-        while (ok && walk.next(t)) {
-            const float* const pa = p.sfa + int64_t(t.row0) * p.k_tiles;
-            const int n_block = t.n0 / 128;
-            for (int k0 = k_begin; k0 < k_end; k0 += kGroupK, ++group) {
-                float a[kRowsA][kGroupK], b[kRowScales ? kRowsB : C::kWeightBlocks][kGroupK];
-#pragma unroll
-                for (int j = 0; j < kRowsA; ++j) load4(pa + int64_t(min(j * 32 + lane, t.valid - 1)) * p.k_tiles, k0, a[j]);
-                if constexpr (kRowScales) {
-#pragma unroll
-                    for (int j = 0; j < kRowsB; ++j) load4(p.sfb + int64_t(min(t.n0 + j * 32 + lane, p.n - 1)) * p.k_tiles, k0, b[j]);
+        } else if (warp == C::kScaleWarp) {
+            // ------------------------------------------------------------ scales
+            // A group's are in registers before its slot is free.  A lane has every 32nd row; four neighbouring k-tiles are one load where
+            // they lie on 16 bytes.
+            constexpr int kRowsA = kTileM / 32, kRowsB = kRowScales ? BN / 32 : 1;
+            const bool wide = p.k_tiles % 4 == 0 && p.wide_scales != 0;
+            const auto load4 = [&](const float* q, int k0, float (&v)[kGroupK]) {
+                if (wide && k0 % 4 == 0 && k0 + kGroupK <= k_end) {
+                    const float4 f = __ldg(reinterpret_cast<const float4*>(q + k0));
+                    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
                 } else {
 #pragma unroll
-                    for (int j = 0; j < C::kWeightBlocks; ++j) {
-                        load4(p.sfb + (int64_t(t.expert) * p.n_blocks + min(n_block + j, p.n_blocks - 1)) * p.k_tiles, k0, b[j]);
-                    }
+                    for (int i = 0; i < kGroupK; ++i) v[i] = k0 + i < k_end ? __ldg(q + k0 + i) : 0.0f;
                 }
-                const uint32_t slot = group % kScaleSlots;
-                ok = wait_bar<C::kRegSplit>(ptx::smem_u32(&bars->sf_empty[slot]), ((group / kScaleSlots) & 1u) ^ 1u, abort, kStatusProducer);
-                if (!ok) break;
-                float* const to = scales + slot * (kGroupK * C::kScales) + lane;
+            };
+            uint32_t group = 0;
+            bool ok = true;
+            BlockWalk<BN, kGrouped> walk(p, tables, first, step);
+            BlockTile t;
+            while (ok && walk.next(t)) {
+                const float* const pa = p.sfa + int64_t(t.row0) * p.k_tiles;
+                const int n_block = t.n0 / 128;
+                for (int k0 = k_begin; k0 < k_end; k0 += kGroupK, ++group) {
+                    float a[kRowsA][kGroupK], b[kRowScales ? kRowsB : C::kWeightBlocks][kGroupK];
 #pragma unroll
-                for (int i = 0; i < kGroupK; ++i) {
-#pragma unroll
-                    for (int j = 0; j < kRowsA; ++j) {
-                        if constexpr (kRowScales) {
-                            to[i * C::kScales + j * 32] = a[j][i];
-                        } else {
-#pragma unroll
-                            for (int h = 0; h < C::kWeightBlocks; ++h) to[i * C::kScales + h * kTileM + j * 32] = a[j][i] * b[h][i];
-                        }
-                    }
+                    for (int j = 0; j < kRowsA; ++j) load4(pa + int64_t(min(j * 32 + lane, t.valid - 1)) * p.k_tiles, k0, a[j]);
                     if constexpr (kRowScales) {
 #pragma unroll
-                        for (int j = 0; j < kRowsB; ++j) to[i * C::kScales + kTileM + j * 32] = b[j][i];
+                        for (int j = 0; j < kRowsB; ++j) load4(p.sfb + int64_t(min(t.n0 + j * 32 + lane, p.n - 1)) * p.k_tiles, k0, b[j]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < C::kWeightBlocks; ++j) {
+                            load4(p.sfb + (int64_t(t.expert) * p.n_blocks + min(n_block + j, p.n_blocks - 1)) * p.k_tiles, k0, b[j]);
+                        }
                     }
+                    const uint32_t slot = group % kScaleSlots;
+                    ok = wait_bar<C::kRegSplit>(ptx::smem_u32(&bars->sf_empty[slot]), ((group / kScaleSlots) & 1u) ^ 1u, abort, kStatusProducer);
+                    if (!ok) break;
+                    float* const to = scales + slot * (kGroupK * C::kScales) + lane;
+#pragma unroll
+                    for (int i = 0; i < kGroupK; ++i) {
+#pragma unroll
+                        for (int j = 0; j < kRowsA; ++j) {
+                            if constexpr (kRowScales) {
+                                to[i * C::kScales + j * 32] = a[j][i];
+                            } else {
+#pragma unroll
+                                for (int h = 0; h < C::kWeightBlocks; ++h) to[i * C::kScales + h * kTileM + j * 32] = a[j][i] * b[h][i];
+                            }
+                        }
+                        if constexpr (kRowScales) {
+#pragma unroll
+                            for (int j = 0; j < kRowsB; ++j) to[i * C::kScales + kTileM + j * 32] = b[j][i];
+                        }
+                    }
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&bars->sf_full[slot]));
                 }
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&bars->sf_full[slot]));
             }
         }
-    }
     } else {
         // ------------------------------------------------------------ promotion and epilogue
         if constexpr (C::kRegSplit) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
