@@ -112,6 +112,8 @@ __global__ void __launch_bounds__(kRowThreads) swiglu_block_quant_kernel(const T
 // A CTA reads and quantises 4096 values of one token, 16 a thread, once and writes them to each of the token's rows.  The blocks
 // behind the tokens write the rows that pad the experts' runs as the codes of zeros.
 
+constexpr int kPadCtas = 16;  // CTAs that share the padding of a run
+
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads) permute_block_quant_kernel(const T* __restrict__ x, int64_t ld, int tokens, int k, int topk,
                                                                           const int* __restrict__ rows, const int* __restrict__ pairs,
@@ -122,7 +124,7 @@ __global__ void __launch_bounds__(kRowThreads) permute_block_quant_kernel(const 
     const int kb = (k + kQBlock - 1) / kQBlock;
     const int c = blockIdx.y * (kRowThreads * 16) + threadIdx.x * 16;
     if (int(blockIdx.x) >= tokens) {
-        const int e = int(blockIdx.x) - tokens;
+        const int pad = int(blockIdx.x) - tokens, e = pad / kPadCtas;
         const BlockScale s = block_scale(0, true);
         // the first row without a pair, by halving
         int first = max(offsets[e], 0);
@@ -131,7 +133,7 @@ __global__ void __launch_bounds__(kRowThreads) permute_block_quant_kernel(const 
             const int half = n / 2;
             if (pairs[first + half] >= 0) first += half + 1, n -= half + 1; else n = half;
         }
-        for (int r = first; r < end; ++r) {
+        for (int r = first + pad % kPadCtas; r < end; r += kPadCtas) {
             if (c < k) {
                 *reinterpret_cast<uint4*>(q + int64_t(r) * k + c) = make_uint4(0, 0, 0, 0);
                 if ((threadIdx.x & 7) == 0) sf[int64_t(r) * kb + c / kQBlock] = s.scale;
@@ -383,7 +385,7 @@ extern "C" int hq_moe_permute_block_quant(const void* input, int64_t ld_elems, i
         return fail(err, errlen, HQ_ERR_INVALID, "input dtype must be bfloat16 or float16");
     }
     if (tokens < 0 || topk < 0 || num_experts < 0 || n_rows < 0 || tokens * topk > INT32_MAX || n_rows > INT32_MAX || num_experts > 65535 ||
-        tokens + num_experts > INT32_MAX) {
+        tokens + num_experts * hq::kPadCtas > INT32_MAX) {
         return fail(err, errlen, HQ_ERR_INVALID, "too many tokens, rows or experts");
     }
     if (k < 0 || k > (int64_t(1) << 22) || k % 16 != 0) {
@@ -401,7 +403,7 @@ extern "C" int hq_moe_permute_block_quant(const void* input, int64_t ld_elems, i
     }
     const hq::DeviceGuard guard(device);
     if (!guard.ok()) return fail(err, errlen, HQ_ERR_CUDA, "cannot select CUDA device %d", device);
-    const dim3 grid(unsigned(tokens + (padded != 0 ? num_experts : 0)), unsigned((k + hq::kRowThreads * 16 - 1) / (hq::kRowThreads * 16)));
+    const dim3 grid(unsigned(tokens + (padded != 0 ? num_experts * hq::kPadCtas : 0)), unsigned((k + hq::kRowThreads * 16 - 1) / (hq::kRowThreads * 16)));
     const auto go = [&](auto kernel, auto* x) {
         return hq::launch(kernel, grid, dim3(hq::kRowThreads), 0, static_cast<cudaStream_t>(stream), use_pdl != 0, 1, x, ld_elems,
                           int(tokens), int(k), int(topk), rows, pairs, offsets, int(n_rows), static_cast<uint8_t*>(out_q),
