@@ -29,8 +29,8 @@ __device__ __forceinline__ uint32_t max8(uint32_t m) {
 }
 
 template <typename T, int kVec>
-__global__ void __launch_bounds__(kRowThreads) block_quant_rows_kernel(const T* __restrict__ x, int64_t ld, int64_t m, int k, int segs,
-                                                                       uint8_t* __restrict__ q, float* __restrict__ sf) {
+__global__ void __launch_bounds__(kRowThreads) block_quant_rows_kernel(const T* x, int64_t ld, int64_t m, int k, int segs,
+                                                                       uint8_t* q, float* sf) {
     grid_wait();
     grid_launch_dependents();
     const int lane = threadIdx.x & 31;
@@ -64,9 +64,9 @@ __global__ void __launch_bounds__(kRowThreads) block_quant_rows_kernel(const T* 
 // Rows from *row_limit on (behind the last expert's run) are left alone.
 
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) swiglu_block_quant_kernel(const T* __restrict__ x, int64_t ld, int64_t m, int k, int segs,
-                                                                         const int* __restrict__ row_limit, uint8_t* __restrict__ q,
-                                                                         float* __restrict__ sf) {
+__global__ void __launch_bounds__(kRowThreads) swiglu_block_quant_kernel(const T* x, int64_t ld, int64_t m, int k, int segs,
+                                                                         const int* row_limit, uint8_t* q,
+                                                                         float* sf) {
     grid_wait();
     grid_launch_dependents();
     const int lane = threadIdx.x & 31;
@@ -115,10 +115,10 @@ __global__ void __launch_bounds__(kRowThreads) swiglu_block_quant_kernel(const T
 constexpr int kPadCtas = 16;  // CTAs that share the padding of a run
 
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) permute_block_quant_kernel(const T* __restrict__ x, int64_t ld, int tokens, int k, int topk,
-                                                                          const int* __restrict__ rows, const int* __restrict__ pairs,
-                                                                          const int* __restrict__ offsets, int n_rows,
-                                                                          uint8_t* __restrict__ q, float* __restrict__ sf) {
+__global__ void __launch_bounds__(kRowThreads) permute_block_quant_kernel(const T* x, int64_t ld, int tokens, int k, int topk,
+                                                                          const int* rows, const int* pairs,
+                                                                          const int* offsets, int n_rows,
+                                                                          uint8_t* q, float* sf) {
     grid_wait();
     grid_launch_dependents();
     const int kb = (k + kQBlock - 1) / kQBlock;
@@ -164,8 +164,8 @@ __global__ void __launch_bounds__(kRowThreads) permute_block_quant_kernel(const 
 // bytes is XORed with the line's thread column: neither side has bank conflicts.
 
 template <typename T, bool kSquare, bool kTranspose>
-__global__ void __launch_bounds__(256) block_quant_tile_kernel(const T* __restrict__ x, int64_t ld, int64_t batch_stride, int64_t m, int k,
-                                                               int64_t m_out, uint8_t* __restrict__ q, float* __restrict__ sf) {
+__global__ void __launch_bounds__(256) block_quant_tile_kernel(const T* x, int64_t ld, int64_t batch_stride, int64_t m, int k,
+                                                               int64_t m_out, uint8_t* q, float* sf) {
     __shared__ uint32_t amax_s[8][64];
     __shared__ float2 factors[kSquare ? 1 : 128];  // of each column: 448 / amax, and whether its block is finite
     __shared__ __align__(16) uint8_t tile[kTranspose ? 128 * 128 : 16];

@@ -258,10 +258,12 @@ int any_dtype(const at::Tensor& t) { return t.scalar_type() == at::kFloat ? HQ_D
 bool rows16(const at::Tensor& x) {
     if (x.stride(-1) != 1 || reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 != 0) return false;
     for (int64_t i = 0; i + 1 < x.dim(); ++i) {
-        if (x.stride(i) % 8 != 0) return false;
+        if (x.size(i) > 1 && x.stride(i) % 8 != 0) return false;
     }
     return true;
 }
+// elements between rows (of a single row: of no consequence, whatever its stride)
+int64_t pitch(const at::Tensor& x, int64_t dim) { return x.size(dim) > 1 ? x.stride(dim) : (x.size(-1) + 7) / 8 * 8; }
 
 // An output that the caller may have given: false if it is not what it should be.
 bool given(PyObject* o, c10::IntArrayRef shape, at::ScalarType type, const at::Tensor& like, at::Tensor* out) {
@@ -342,7 +344,7 @@ PyObject* block_quant(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     at::Tensor q, sf;
     if (!given(a[4], qs, at::kFloat8_e4m3fn, *x, &q) || !given(a[5], ss, at::kFloat, *x, &sf)) Py_RETURN_NONE;
     const void* const px = x->data_ptr();
-    const int64_t ld = x->stride(-2), batch = x->dim() == 3 ? x->stride(0) : 0;
+    const int64_t ld = pitch(*x, -2), batch = x->dim() == 3 ? pitch(*x, 0) : 0;
     const int dev = x->get_device();
     void* const st = stream_of(*x);
     const c10::Device device = x->device();
@@ -381,7 +383,7 @@ PyObject* swiglu_block_quant(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     at::Tensor q, sf;
     if (!given(a[3], qs, at::kFloat8_e4m3fn, *x, &q) || !given(a[4], ss, at::kFloat, *x, &sf)) Py_RETURN_NONE;
     const void* const px = x->data_ptr();
-    const int64_t ld = x->stride(0);
+    const int64_t ld = pitch(*x, 0);
     const int dev = x->get_device();
     void* const st = stream_of(*x);
     const c10::Device device = x->device();
@@ -567,7 +569,7 @@ PyObject* moe_permute_block_quant(PyObject*, PyObject* const* a, Py_ssize_t narg
     at::Tensor q, sf;
     if (!given(a[3], qs, at::kFloat8_e4m3fn, *x, &q) || !given(a[4], ss, at::kFloat, *x, &sf)) Py_RETURN_NONE;
     const void* const px = x->data_ptr();
-    const int64_t ld = x->stride(0);
+    const int64_t ld = pitch(*x, 0);
     const int dev = x->get_device();
     void* const st = stream_of(*x);
     const c10::Device device = x->device();

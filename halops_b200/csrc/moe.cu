@@ -23,6 +23,7 @@
 namespace hq {
 namespace {
 
+// No kernel pointer here is __restrict__: what it points to changes, in the preceding kernel, while this one waits for it.
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
@@ -46,9 +47,9 @@ __device__ __forceinline__ int expert_of(const Id* ids, int p, int pairs_n, int 
 }
 
 template <typename Id>
-__global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const Id* __restrict__ ids, int pairs_n, int experts, int align, int n_rows,
-                                                                int ctas, int* __restrict__ rows, int* __restrict__ pairs,
-                                                                int* __restrict__ offsets, int* __restrict__ expert_ids) {
+__global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const Id* ids, int pairs_n, int experts, int align, int n_rows,
+                                                                int ctas, int* rows, int* pairs,
+                                                                int* offsets, int* expert_ids) {
     extern __shared__ int smem[];
     int* const lines = smem;                             // [warp][expert]
     int* const total = lines + kSortWarps * experts;     // this CTA's pairs per expert, read by the cluster
@@ -208,9 +209,9 @@ __device__ __forceinline__ void padding_of(const int* pairs, const int* offsets,
 constexpr int kMoveThreads = 256;
 
 template <typename Unit, int kPer>
-__global__ void __launch_bounds__(kMoveThreads) moe_permute_kernel(const Unit* __restrict__ x, int64_t ld, int tokens, int units, int topk,
-                                                                   const int* __restrict__ rows, const int* __restrict__ pairs,
-                                                                   const int* __restrict__ offsets, int n_rows, Unit* __restrict__ out) {
+__global__ void __launch_bounds__(kMoveThreads) moe_permute_kernel(const Unit* x, int64_t ld, int tokens, int units, int topk,
+                                                                   const int* rows, const int* pairs,
+                                                                   const int* offsets, int n_rows, Unit* out) {
     grid_wait();
     grid_launch_dependents();
     const int c = blockIdx.y * (kMoveThreads * kPer) + threadIdx.x;
@@ -230,7 +231,7 @@ __global__ void __launch_bounds__(kMoveThreads) moe_permute_kernel(const Unit* _
     Unit v[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        if (c + i * kMoveThreads < units) v[i] = x[token * ld + c + i * kMoveThreads];
+        if (c + i * kMoveThreads < units) v[i] = __ldg(x + token * ld + c + i * kMoveThreads);
     }
     for (int j0 = 0; j0 < topk; j0 += 8) {
         int r[8];
@@ -370,9 +371,9 @@ struct Piece<T, 2> {
 };
 
 template <typename T, int kBytes, int kPer>
-__global__ void __launch_bounds__(kMoveThreads) moe_unpermute_kernel(const T* __restrict__ z, int64_t ld, int tokens, int h, int topk,
-                                                                     const int* __restrict__ rows, int n_rows,
-                                                                     const float* __restrict__ weights, T* __restrict__ y) {
+__global__ void __launch_bounds__(kMoveThreads) moe_unpermute_kernel(const T* z, int64_t ld, int tokens, int h, int topk,
+                                                                     const int* rows, int n_rows,
+                                                                     const float* weights, T* y) {
     using P = Piece<T, kBytes>;
     constexpr int kSlots = 4;  // rows loaded before the first is added
     grid_wait();
@@ -429,9 +430,9 @@ __global__ void __launch_bounds__(kMoveThreads) moe_unpermute_kernel(const T* __
 // neighbours, so that its gradient comes from HBM once.  The CTAs behind the pairs zero the rows that pad the runs.
 template <typename T, int kBytes, int kGroup>
 __global__ void __launch_bounds__(kMoveThreads) moe_unpermute_backward_kernel(
-    const T* __restrict__ gy, int64_t ld_g, const T* __restrict__ z, int64_t ld_z, int pairs_n, int pair_ctas, int h, int topk,
-    const int* __restrict__ rows, const int* __restrict__ pairs, const int* __restrict__ offsets, int n_rows,
-    const float* __restrict__ weights, T* __restrict__ gz, float* __restrict__ gw) {
+    const T* gy, int64_t ld_g, const T* z, int64_t ld_z, int pairs_n, int pair_ctas, int h, int topk,
+    const int* rows, const int* pairs, const int* offsets, int n_rows,
+    const float* weights, T* gz, float* gw) {
     using P = Piece<T, kBytes>;
     constexpr int kAhead = kBytes == 16 ? 4 : 8, kStep = kGroup * P::kN;
     __shared__ float parts[kMoveThreads / 32];

@@ -48,7 +48,13 @@ def _on_device(device: torch.device, **tensors) -> None:
 
 def _rows_ok(t: torch.Tensor) -> bool:
     """16-bit rows that the kernels can read: contiguous, on 16 bytes."""
-    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1])
+    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
+            and all(s % 8 == 0 or n <= 1 for s, n in zip(t.stride()[:-1], t.shape[:-1])))
+
+
+def _pitch(t: torch.Tensor, dim: int = -2) -> int:
+    """Elements between rows (of a single row: of no consequence, whatever its stride)."""
+    return t.stride(dim) if t.size(dim) > 1 else (t.size(-1) + 7) // 8 * 8
 
 
 def _quant_outputs(q, sf, q_shape, sf_shape, device):
@@ -108,7 +114,7 @@ def block_quant(
     q, sf = _quant_outputs(output_quant, output_sf, q_shape, sf_shape, input.device)
     _on_device(input.device, input=input)
     _native.call(
-        "hq_block_quant", input.data_ptr(), input.stride(-2), input.stride(0) if input.dim() == 3 else 0, _IN_DTYPES[input.dtype],
+        "hq_block_quant", input.data_ptr(), _pitch(input), _pitch(input, 0) if input.dim() == 3 else 0, _IN_DTYPES[input.dtype],
         input.size(0) if input.dim() == 3 else 1, m, k, block[0], int(bool(transpose)), int(bool(use_pdl)), q.data_ptr(),
         sf.data_ptr(), input.device.index, _native.current_stream(input.device))
     return q, sf
@@ -147,7 +153,7 @@ def swiglu_block_quant(
     _on_device(input.device, input=input, offsets=offsets)
     limit = None if offsets is None else offsets.data_ptr() + 4 * (offsets.size(0) - 1)
     _native.call(
-        "hq_swiglu_block_quant", input.data_ptr(), input.stride(0), _IN_DTYPES[input.dtype], m, k, limit, int(bool(use_pdl)),
+        "hq_swiglu_block_quant", input.data_ptr(), _pitch(input), _IN_DTYPES[input.dtype], m, k, limit, int(bool(use_pdl)),
         q.data_ptr(), sf.data_ptr(), input.device.index, _native.current_stream(input.device))
     return q, sf
 

@@ -22,7 +22,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from . import _native
-from .gemm.block_scale import _IN_DTYPES, _OUT_DTYPES, _blocks, _check, _on_device, _quant_outputs, _rows_ok
+from .gemm.block_scale import _IN_DTYPES, _OUT_DTYPES, _blocks, _check, _on_device, _pitch, _quant_outputs, _rows_ok
 
 __all__ = ["MoeSort", "moe_permute", "moe_permute_backward", "moe_permute_block_quant", "moe_sort", "moe_unpermute",
            "moe_unpermute_backward"]
@@ -150,7 +150,7 @@ def moe_permute_block_quant(
     _check(input.size(0) == tokens, f"input must have the sort's {tokens} tokens, got {input.size(0)}")
     q, sf = _quant_outputs(output_quant, output_sf, (n_rows, h), (n_rows, _blocks(h)), input.device)
     _on_device(input.device, input=input)
-    _native.call("hq_moe_permute_block_quant", input.data_ptr(), input.stride(0), _IN_DTYPES[input.dtype], tokens, h, topk,
+    _native.call("hq_moe_permute_block_quant", input.data_ptr(), _pitch(input), _IN_DTYPES[input.dtype], tokens, h, topk,
                  sort.rows.data_ptr(), sort.pairs.data_ptr(), sort.offsets.data_ptr(), experts, n_rows, int(sort.align > 1),
                  int(bool(use_pdl)), q.data_ptr(), sf.data_ptr(), input.device.index, _native.current_stream(input.device))
     return q, sf

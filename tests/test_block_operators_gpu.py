@@ -201,3 +201,58 @@ def test_outputs_do_not_share_what_they_are_kept_by(hq):
     torch.cuda.synchronize()
     junk = [torch.full((1 << 16,), 7, dtype=torch.uint8, device="cuda") for _ in range(50)]
     assert torch.equal(sf, keep) and sf.is_contiguous() and junk[0][0] == 7
+
+
+def test_a_single_row_may_have_any_stride(hq, monkeypatch):
+    from halops_b200 import _native
+
+    _native.load_fast_path()
+    column = torch.randn(256, 1, device="cuda").to(BF16)
+    row = column.t()
+    assert row.shape == (1, 256) and row.stride(0) == 1
+    order = hq.moe_sort(torch.tensor([[0, 1]], device="cuda"), 2)
+    for front in (_native.fast_path, _native._NoFastPath):
+        monkeypatch.setattr(_native, "fast_path", front)
+        whole = row.contiguous().clone()
+        for block, transpose in (((1, 128), False), ((1, 128), True), ((128, 128), False), ((128, 128), True)):
+            got, want = hq.block_quant(row, block, transpose), hq.block_quant(whole, block, transpose)
+            assert _same(got[0], want[0]) and torch.equal(got[1], want[1])
+        got, want = hq.swiglu_block_quant(row), hq.swiglu_block_quant(whole)
+        assert _same(got[0], want[0]) and torch.equal(got[1], want[1])
+        got, want = hq.moe_permute_block_quant(row, order), hq.moe_permute_block_quant(whole, order)
+        assert _same(got[0], want[0]) and torch.equal(got[1], want[1])
+        assert torch.equal(hq.moe_permute(row, order), hq.moe_permute(whole, order))
+        assert torch.equal(hq.moe_permute(row.expand(1, 256), order), hq.moe_permute(whole, order))
+
+
+def test_results_of_the_preceding_kernel_are_waited_for(hq):
+    """Programmatic launches back to back, each on what the one before wrote into the same buffers."""
+    tokens, topk, h = 512, 2, 256
+    ids = torch.empty(tokens, topk, dtype=torch.int64, device="cuda")
+    x = torch.empty(tokens, h, dtype=BF16, device="cuda")
+    w = torch.randn(4, 128, h, device="cuda").to(BF16)
+    wq, ws = hq.block_quant(w, (128, 128))
+    out = torch.empty(tokens * topk, 128, dtype=BF16, device="cuda")
+    q, sf = torch.empty(tokens * topk, h, dtype=torch.float8_e4m3fn, device="cuda"), torch.empty(tokens * topk, h // 128, device="cuda")
+    inputs = [(torch.randint(0, 4, (tokens, topk), device="cuda"), torch.randn(tokens, h, device="cuda").to(BF16)) for _ in range(8)]
+
+    def step(pdl):
+        order = hq.moe_sort(ids, 4, use_pdl=pdl)
+        hq.moe_permute_block_quant(x, order, use_pdl=pdl, output_quant=q, output_sf=sf)
+        hq.group_block_gemm(q, wq, sf, ws, order.offsets, out, use_pdl=pdl)
+        return hq.moe_unpermute(out, order, use_pdl=pdl)
+
+    want = []
+    for i, v in inputs:
+        ids.copy_(i)
+        x.copy_(v)
+        torch.cuda.synchronize()
+        want.append(step(False))
+        torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for i, v in inputs:
+            ids.copy_(i)
+            x.copy_(v)
+            got.append(step(True))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
