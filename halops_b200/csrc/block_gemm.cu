@@ -14,13 +14,12 @@
 //               threads that use them, a float of a row each, they took a sixth of the time: 8192 x 8192 x 8192 625 us, 537 without)
 //   1 or 2 warps  issue the MMAs of a step (BN > 128: one block; else two, one each) into the next of 2 sets of buffers in tensor memory
 //
-// What bounds it.  A step is a round between the roles: MMAs (512 cycles on 256 columns), commit and wake-up (100), loads and products of
-// the promotion (about 70 cycles for each 16 columns of its two warps a scheduler, which wait for the loads together: 560), the signal back
-// (100 to 200); with two sets of buffers half of that is hidden, 850 to 870 cycles a block.  The tensor pipe is busy for half of
-// the time (ncu: 52 % on 4096 x 7168 x 2048), L2 for a third.  Large problems run at the power cap besides: 8192 x 8192 x 8192 takes 545 to
-// 605 us at 1.38 GHz and 990 W (the MXFP8 kernel, whose scales cost no such round, 432 at 1.17).  Measured and left: 16 promotion warps on 256
-// columns (registers spill; 595 us against 540), double-buffered loads (648), half of B's bytes, as a CTA pair would load (518 without what
-// a pair's remote signals would add).
+// What bounds it.  A k-tile of 256 columns takes 850 to 870 cycles, 512 of them MMAs (ncu: the tensor pipe busy for 52 % of 4096 x 7168 x 2048, L2
+// and the way from it for a third, issue slots for 39 %).  Without the promotion's products it takes 640 to 670; the rest is the round of
+// the promotion (287 cycles of loads and 260 of products, one after the other in warps that wait together).  Large problems run
+// at the power cap besides: 8192 x 8192 x 8192 takes 545 to 605 us at 1.38 GHz and 990 W (the MXFP8 kernel 432 at 1.17).  Measured and left:
+// 16 promotion warps on 256 columns (registers spill; 595 us against 540), double-buffered loads (648), half of B's bytes, as a CTA pair
+// would load (518, without what a pair's remote signals would add).
 //
 // Every mbarrier wait is bounded, as in the other GEMM kernels: a role that waits longer than kTimeoutNs records a code in the
 // status word, raises the CTA's abort flag and all roles leave through the common teardown.
@@ -304,6 +303,46 @@ __device__ __forceinline__ void store_values(const float (&f)[kN], void* out, in
     }
 }
 
+// ---------------------------------------------------------------------------- MMA issuers
+//
+// One for each k-tile of a step.  Every k-tile has a buffer of its own, so nothing has to be kept in order between them.  (Two that took
+// turns at the steps would skip phases of the stages' barriers, and a wait for the next but one is over before it began.)  kU, the issuer's
+// k-tile, is known at compile time and every instruction elected for itself (the same mask elects the same lane each time, so a commit
+// follows the MMAs of its own thread), which keeps the operands warp-uniform: 4736 x 768 x 4096 on 64 columns 22.9 -> 21.6 us, 4736 x 1024 x
+// 4096 on 128 22.8 -> 22.3.  (A half of the 256 columns for each of two issuers, with buffers and
+// signals of its own: no faster.)
+template <int BN, bool kRowScales, bool kGrouped, int kU>
+__device__ __forceinline__ void issue_mmas(const BlockArgs& p, const int* tables, int first, int step, int k_begin, int k_end, BlockBars* bars,
+                                           volatile uint32_t* abort, uint32_t a_base, uint32_t b_base, uint32_t tmem) {
+    using C = BlockCfg<BN, kRowScales>;
+    // float32 sums, e4m3 operands, both K-major; N >> 3, M >> 4
+    constexpr uint32_t idesc = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(kTileM >> 4) << 24);
+    // (addresses are in the descriptors' low bits, in units of 16 bytes; K = 32 bytes is a step of 2 inside of the swizzle atom)
+    const uint64_t adesc0 = ptx::smem_desc(a_base + kU * C::kABytes, 16, 1024, 2);
+    const uint64_t bdesc0 = ptx::smem_desc(b_base + kU * C::kBBytes, 16, 1024, 2);
+    uint32_t it = 0;
+    bool ok = true;
+    BlockWalk<BN, kGrouped> walk(p, tables, first, step);
+    BlockTile t;
+    while (ok && walk.next(t)) {
+        for (int kt = k_begin; kt < k_end; kt += C::kStep, ++it) {
+            const uint32_t s = it % C::kStages, buf = it % C::kBufs;
+            ok = wait_bars<C::kRegSplit>(ptx::smem_u32(&bars->full[s]), (it / C::kStages) & 1u, true, ptx::smem_u32(&bars->acc_empty[buf]),
+                                         ((it / C::kBufs) & 1u) ^ 1u, abort, kStatusMma);
+            if (!ok) break;
+            ptx::tc_fence_after();
+            const uint64_t adesc = adesc0 + s * (C::kStep * C::kABytes >> 4), bdesc = bdesc0 + s * (C::kStep * C::kBBytes >> 4);
+            const uint32_t d = tmem + (buf * C::kStep + kU) * BN;
+            if (ptx::elect_one()) mma_e4m3(d, adesc, bdesc, idesc, 0u);
+            if (ptx::elect_one()) mma_e4m3(d, adesc + 2, bdesc + 2, idesc, 1u);
+            if (ptx::elect_one()) mma_e4m3(d, adesc + 4, bdesc + 4, idesc, 1u);
+            if (ptx::elect_one()) mma_e4m3(d, adesc + 6, bdesc + 6, idesc, 1u);
+            if (ptx::elect_one()) ptx::tc_commit(ptx::smem_u32(&bars->acc_full[buf]));
+            if (ptx::elect_one()) ptx::tc_commit(ptx::smem_u32(&bars->empty[s]));
+        }
+    }
+}
+
 // kAnyRows: output rows on no 16 bytes.  (An instantiation of its own: as a branch it cost the 256-wide tile registers, 8192 x 8192 x 8192
 // 580 -> 615 us.)
 template <int BN, bool kRowScales, bool kGrouped, bool kSplit, bool kAnyRows>
@@ -449,38 +488,10 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
             for (uint32_t d = it > uint32_t(C::kStages) ? it - C::kStages : 0u; ok && d < it; ++d) {
                 ok = wait_bar<C::kRegSplit>(ptx::smem_u32(&bars->empty[d % C::kStages]), (d / C::kStages) & 1u, abort, kStatusProducer);
             }
-        } else if (warp >= C::kMmaWarp && warp < C::kMmaWarp + C::kStep) {
-            // ------------------------------------------------------------ MMA issuers
-            // One for each k-tile of a step.  Every k-tile has a buffer of its own, so nothing has to be kept in order between them.  (Two that took
-            // turns at the steps would skip phases of the stages' barriers, and a wait for the next but one is over before it began.)
-            // float32 sums, e4m3 operands, both K-major; N >> 3, M >> 4
-            constexpr uint32_t idesc = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(kTileM >> 4) << 24);
-            const uint32_t u = warp - C::kMmaWarp;
-            const uint64_t adesc0 = ptx::smem_desc(a_base, 16, 1024, 2), bdesc0 = ptx::smem_desc(b_base, 16, 1024, 2);
-            uint32_t it = 0;
-            bool ok = true;
-            BlockWalk<BN, kGrouped> walk(p, tables, first, step);
-            BlockTile t;
-            while (ok && walk.next(t)) {
-                for (int kt = k_begin; kt < k_end; kt += C::kStep, ++it) {
-                    const uint32_t s = it % C::kStages, buf = it % C::kBufs;
-                    ok = wait_bars<C::kRegSplit>(ptx::smem_u32(&bars->full[s]), (it / C::kStages) & 1u, true, ptx::smem_u32(&bars->acc_empty[buf]),
-                                   ((it / C::kBufs) & 1u) ^ 1u, abort, kStatusMma);
-                    if (!ok) break;
-                    ptx::tc_fence_after();
-                    // (addresses are in the descriptors' low bits, in units of 16 bytes; K = 32 bytes is a step of 2 inside of the swizzle atom)
-                    const uint64_t adesc = adesc0 + (s * C::kStep + u) * (C::kABytes >> 4), bdesc = bdesc0 + (s * C::kStep + u) * (C::kBBytes >> 4);
-                    const uint32_t d = tmem + (buf * C::kStep + u) * BN;
-                    if (ptx::elect_one()) {
-                        mma_e4m3(d, adesc, bdesc, idesc, 0u);
-                        mma_e4m3(d, adesc + 2, bdesc + 2, idesc, 1u);
-                        mma_e4m3(d, adesc + 4, bdesc + 4, idesc, 1u);
-                        mma_e4m3(d, adesc + 6, bdesc + 6, idesc, 1u);
-                        ptx::tc_commit(ptx::smem_u32(&bars->acc_full[buf]));
-                        ptx::tc_commit(ptx::smem_u32(&bars->empty[s]));
-                    }
-                }
-            }
+        } else if (warp == C::kMmaWarp) {
+            issue_mmas<BN, kRowScales, kGrouped, 0>(p, tables, first, step, k_begin, k_end, bars, abort, a_base, b_base, tmem);
+        } else if (C::kStep == 2 && warp == C::kMmaWarp + 1) {
+            issue_mmas<BN, kRowScales, kGrouped, 1>(p, tables, first, step, k_begin, k_end, bars, abort, a_base, b_base, tmem);
         } else if (warp == C::kScaleWarp) {
             // ------------------------------------------------------------ scales
             // A group's are in registers before its slot is free.  A lane has every 32nd row; four neighbouring k-tiles are one load where
