@@ -306,20 +306,23 @@ __device__ __forceinline__ void store_values(const float (&f)[kN], void* out, in
 // ---------------------------------------------------------------------------- MMA issuers
 //
 // One for each k-tile of a step.  Every k-tile has a buffer of its own, so nothing has to be kept in order between them.  (Two that took
-// turns at the steps would skip phases of the stages' barriers, and a wait for the next but one is over before it began.)  kU, the issuer's
-// k-tile, is known at compile time and every instruction elected for itself (the same mask elects the same lane each time, so a commit
-// follows the MMAs of its own thread), which keeps the operands warp-uniform: 4736 x 768 x 4096 on 64 columns 22.9 -> 21.6 us, 4736 x 1024 x
-// 4096 on 128 22.8 -> 22.3.  (A half of the 256 columns for each of two issuers, with buffers and
-// signals of its own: no faster.)
-template <int BN, bool kRowScales, bool kGrouped, int kU>
+// turns at the steps would skip phases of the stages' barriers, and a wait for the next but one is over before it began.)
+//
+// kEach: an issuer's k-tile u is a constant and every instruction elected for itself, which keeps its operands warp-uniform (the same mask
+// elects the same lane each time, so a commit follows the MMAs of its own thread).  It is for tiles of up to 128 columns with scales of
+// blocks, where the round between the roles counts most: 4736 x 768 x 4096 on 64 columns 22.7 -> 21.1 us, 4736 x 1024 x 4096 on 128 23.3 ->
+// 22.9, 1 x 7168 x 2048 5.8 -> 5.3.  Wide tiles and scales of rows have one copy of the loop and one election a step: 7168 x 2048 x 4096
+// 73.4 us against 74.8, 1024 x 2048 x 256 with scales of rows 7.0 against 7.2.  (A half of 256 columns for each of two issuers, with
+// buffers and signals of its own: no faster.)
+template <int BN, bool kRowScales, bool kGrouped, bool kEach>
 __device__ __forceinline__ void issue_mmas(const BlockArgs& p, const int* tables, int first, int step, int k_begin, int k_end, BlockBars* bars,
-                                           volatile uint32_t* abort, uint32_t a_base, uint32_t b_base, uint32_t tmem) {
+                                           volatile uint32_t* abort, uint32_t a_base, uint32_t b_base, uint32_t tmem, uint32_t u) {
     using C = BlockCfg<BN, kRowScales>;
     // float32 sums, e4m3 operands, both K-major; N >> 3, M >> 4
     constexpr uint32_t idesc = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(kTileM >> 4) << 24);
     // (addresses are in the descriptors' low bits, in units of 16 bytes; K = 32 bytes is a step of 2 inside of the swizzle atom)
-    const uint64_t adesc0 = ptx::smem_desc(a_base + kU * C::kABytes, 16, 1024, 2);
-    const uint64_t bdesc0 = ptx::smem_desc(b_base + kU * C::kBBytes, 16, 1024, 2);
+    const uint64_t adesc0 = ptx::smem_desc(a_base + u * C::kABytes, 16, 1024, 2);
+    const uint64_t bdesc0 = ptx::smem_desc(b_base + u * C::kBBytes, 16, 1024, 2);
     uint32_t it = 0;
     bool ok = true;
     BlockWalk<BN, kGrouped> walk(p, tables, first, step);
@@ -332,13 +335,22 @@ __device__ __forceinline__ void issue_mmas(const BlockArgs& p, const int* tables
             if (!ok) break;
             ptx::tc_fence_after();
             const uint64_t adesc = adesc0 + s * (C::kStep * C::kABytes >> 4), bdesc = bdesc0 + s * (C::kStep * C::kBBytes >> 4);
-            const uint32_t d = tmem + (buf * C::kStep + kU) * BN;
-            if (ptx::elect_one()) mma_e4m3(d, adesc, bdesc, idesc, 0u);
-            if (ptx::elect_one()) mma_e4m3(d, adesc + 2, bdesc + 2, idesc, 1u);
-            if (ptx::elect_one()) mma_e4m3(d, adesc + 4, bdesc + 4, idesc, 1u);
-            if (ptx::elect_one()) mma_e4m3(d, adesc + 6, bdesc + 6, idesc, 1u);
-            if (ptx::elect_one()) ptx::tc_commit(ptx::smem_u32(&bars->acc_full[buf]));
-            if (ptx::elect_one()) ptx::tc_commit(ptx::smem_u32(&bars->empty[s]));
+            const uint32_t d = tmem + (buf * C::kStep + u) * BN;
+            if constexpr (kEach) {
+                if (ptx::elect_one()) mma_e4m3(d, adesc, bdesc, idesc, 0u);
+                if (ptx::elect_one()) mma_e4m3(d, adesc + 2, bdesc + 2, idesc, 1u);
+                if (ptx::elect_one()) mma_e4m3(d, adesc + 4, bdesc + 4, idesc, 1u);
+                if (ptx::elect_one()) mma_e4m3(d, adesc + 6, bdesc + 6, idesc, 1u);
+                if (ptx::elect_one()) ptx::tc_commit(ptx::smem_u32(&bars->acc_full[buf]));
+                if (ptx::elect_one()) ptx::tc_commit(ptx::smem_u32(&bars->empty[s]));
+            } else if (ptx::elect_one()) {
+                mma_e4m3(d, adesc, bdesc, idesc, 0u);
+                mma_e4m3(d, adesc + 2, bdesc + 2, idesc, 1u);
+                mma_e4m3(d, adesc + 4, bdesc + 4, idesc, 1u);
+                mma_e4m3(d, adesc + 6, bdesc + 6, idesc, 1u);
+                ptx::tc_commit(ptx::smem_u32(&bars->acc_full[buf]));
+                ptx::tc_commit(ptx::smem_u32(&bars->empty[s]));
+            }
         }
     }
 }
@@ -488,10 +500,14 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
             for (uint32_t d = it > uint32_t(C::kStages) ? it - C::kStages : 0u; ok && d < it; ++d) {
                 ok = wait_bar<C::kRegSplit>(ptx::smem_u32(&bars->empty[d % C::kStages]), (d / C::kStages) & 1u, abort, kStatusProducer);
             }
-        } else if (warp == C::kMmaWarp) {
-            issue_mmas<BN, kRowScales, kGrouped, 0>(p, tables, first, step, k_begin, k_end, bars, abort, a_base, b_base, tmem);
-        } else if (C::kStep == 2 && warp == C::kMmaWarp + 1) {
-            issue_mmas<BN, kRowScales, kGrouped, 1>(p, tables, first, step, k_begin, k_end, bars, abort, a_base, b_base, tmem);
+        } else if (warp >= C::kMmaWarp && warp < C::kMmaWarp + C::kStep) {
+            constexpr bool kEach = C::kStep == 2 && !kRowScales;
+            if (kEach && warp == C::kMmaWarp) {
+                issue_mmas<BN, kRowScales, kGrouped, kEach>(p, tables, first, step, k_begin, k_end, bars, abort, a_base, b_base, tmem, 0u);
+            } else {
+                const uint32_t u = kEach ? 1u : warp - C::kMmaWarp;
+                issue_mmas<BN, kRowScales, kGrouped, kEach>(p, tables, first, step, k_begin, k_end, bars, abort, a_base, b_base, tmem, u);
+            }
         } else if (warp == C::kScaleWarp) {
             // ------------------------------------------------------------ scales
             // A group's are in registers before its slot is free.  A lane has every 32nd row; four neighbouring k-tiles are one load where
