@@ -693,54 +693,68 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
                 }
             } else if constexpr (kAnyRows) {
                 // Rows on no 16 bytes: 64 bytes of 32 rows at a time through the warp's slot, from where neighbouring lanes store neighbouring
-                // words.  (Each thread its row's values one by one: 5776 x 4740 x 5024 377 us, so 190.)
+                // words.  8 loads before their stores: 8192 x 8190 x 2048 220 -> 187 us, 2631 x 2505 x 1872 29.2 -> 24.4 (with TMA stores,
+                // 2631 x 2504 x 1872 takes 22.3).  (Each thread its row's values one by one: twice the time of 5776 x 4740 x 5024, 167.)
                 if (busy) {
                     const uint32_t slot = epi_base + warp * (C::kEpiSlots * 2048);
                     const bool f32 = p.out_type == HQ_DTYPE_FP32;
                     const int rows = min(32, t.valid - quarter * 32);
                     const int64_t row0 = t.row0 + quarter * 32;
-#pragma unroll
-                    for (int c = 0; c < C::kCols; c += 16) {
-                        const int col = t.n0 + part * C::kCols + c;
-                        if (col >= p.n) break;
+                    // lanes of `bytes` each have one row's 64
+                    const int bytes = f32 || p.out_align >= 4 ? 4 : 2, lanes = 64 / bytes, size = f32 ? 4 : 2, per = 32 / lanes;
+                    const int at = lane % lanes * bytes, first = at / size, mine = lane / lanes;
+                    const auto store_rows = [&](int col) {
                         __syncwarp();
+                        const int left = p.n - col - first;
+                        char* to = static_cast<char*>(p.out) + ((row0 + mine) * p.ldo + col + first) * size;
+                        const int64_t next = int64_t(per) * p.ldo * size;
+                        for (int r0 = mine; r0 < rows; r0 += 8 * per) {
+                            uint32_t w[8];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint32_t to = slot + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4);
-                            uint32_t w[4];
-                            if (f32) {
-#pragma unroll
-                                for (int l = 0; l < 4; ++l) w[l] = __float_as_uint(acc[c + j * 4 + l]);
-                            } else if (j < 2) {
-#pragma unroll
-                                for (int l = 0; l < 4; ++l) w[l] = pack16(acc[c + j * 8 + 2 * l], acc[c + j * 8 + 2 * l + 1], p.out_type);
-                            } else {
-                                continue;
+                            for (int i = 0; i < 8; ++i) {
+                                const int r = r0 + i * per;  // (below 32)
+                                const uint32_t from = slot + r * 64 + (((at >> 4) ^ ((r >> 1) & 3)) << 4) + (at & 12);
+                                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[i]) : "r"(from) : "memory");
+                                if (at & 2) w[i] >>= 16;
                             }
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+#pragma unroll
+                            for (int i = 0; i < 8; ++i, to += next) {
+                                if (r0 + i * per >= rows || left <= 0) continue;
+                                if (bytes == 4 && (f32 || left > 1)) {
+                                    *reinterpret_cast<uint32_t*>(to) = w[i];
+                                } else {
+                                    *reinterpret_cast<uint16_t*>(to) = uint16_t(w[i]);
+                                }
+                            }
                         }
                         __syncwarp();
-                        // 16 values of a row: 16 lanes one each (float32, or rows on 2 bytes), or 8 lanes two each
-                        const int lanes = !f32 && p.out_align >= 4 ? 8 : 16, bytes = f32 || p.out_align >= 4 ? 4 : 2;
-                        const int at = lane % lanes * bytes, first = lane % lanes * (16 / lanes), left = p.n - col - first;
-                        for (int r = lane / lanes; r < rows; r += 32 / lanes) {
-                            const uint32_t from = slot + r * 64 + (((at >> 4) ^ ((r >> 1) & 3)) << 4) + (at & 15);
-                            const int64_t o = (row0 + r) * p.ldo + col + first;
-                            if (bytes == 4) {
-                                uint32_t w;
-                                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(from) : "memory");
-                                if (f32) {
-                                    if (left > 0) static_cast<uint32_t*>(p.out)[o] = w;
-                                } else if (left > 1) {
-                                    *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + o) = w;
-                                } else if (left > 0) {
-                                    static_cast<uint16_t*>(p.out)[o] = uint16_t(w);
+                    };
+#pragma unroll
+                    for (int c = 0; c < C::kCols; c += 32) {
+                        const int col = t.n0 + part * C::kCols + c;
+                        if (col >= p.n) break;
+                        if (f32) {
+#pragma unroll
+                            for (int h = 0; h < 32; h += 16) {
+                                if (col + h >= p.n) break;
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    const float* const f = acc + c + h + j * 4;
+                                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(slot + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)),
+                                                 "r"(__float_as_uint(f[0])), "r"(__float_as_uint(f[1])), "r"(__float_as_uint(f[2])),
+                                                 "r"(__float_as_uint(f[3])) : "memory");
                                 }
-                            } else {
-                                uint16_t w;
-                                asm volatile("ld.shared.b16 %0, [%1];" : "=h"(w) : "r"(from) : "memory");
-                                if (left > 0) static_cast<uint16_t*>(p.out)[o] = w;
+                                store_rows(col + h);
                             }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const float* const f = acc + c + j * 8;
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(slot + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)),
+                                             "r"(pack16(f[0], f[1], p.out_type)), "r"(pack16(f[2], f[3], p.out_type)),
+                                             "r"(pack16(f[4], f[5], p.out_type)), "r"(pack16(f[6], f[7], p.out_type)) : "memory");
+                            }
+                            store_rows(col);
                         }
                     }
                 }
