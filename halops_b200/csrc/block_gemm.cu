@@ -88,6 +88,7 @@ struct BlockCfg {
     static constexpr bool kRegSplit = BN == 256;
     static_assert(sizeof(BlockBars) <= kBarBytes && kStages >= 3 && kStages <= 8 && kTmemCols <= 512, "budgets");
     static_assert(BN > 128 || kTileM * (BN + 4) * 4 <= kStages * kStageBytes, "split-K partial sums fit into the ring");
+    static_assert(kRowScales || kCols / 32 % kEpiSlots == 0, "a tile's pieces go round the slots as a whole");
 };
 
 struct BlockArgs {
@@ -765,7 +766,12 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
 #pragma unroll
                 for (int c = 0; c < C::kCols; c += 32) {
                     const int col = t.n0 + part * C::kCols + c;
-                    if (col >= p.n) break;
+                    if (col >= p.n) {
+                        // A group without a store: every tile commits one for each of its pieces, so that a slot's last store is always
+                        // kEpiSlots groups back, also on the tile behind one that sticks out beyond N.
+                        if (lane == 0) ptx::bulk_commit();
+                        continue;
+                    }
                     const uint32_t slot = slots + c / 32 % C::kEpiSlots * 2048;
                     // the store that last read this slot (of this tile, or the one before) is done with it
                     if (lane == 0) ptx::bulk_wait_read<C::kEpiSlots - 1>();
