@@ -42,7 +42,7 @@ __all__ = ["EpilogueOp", "MoeSort", "batch_gemm", "block_gemm", "block_quant", "
            "group_contiguous_gemm", "group_masked_gemm", "group_wise_quant", "interleave_gate_up", "low_latency_mma_gemm",
            "moe_permute", "moe_permute_backward", "moe_permute_block_quant", "moe_sort", "moe_unpermute",
            "moe_unpermute_backward", "rms_norm_quant", "swiglu_block_quant", "device_status", "selftest_bounded_wait", "describe_tile",
-           "describe_group_tile", "lib_path"]
+           "describe_block_tile", "describe_group_tile", "lib_path"]
 __version__ = "0.1.0"
 
 
@@ -85,6 +85,21 @@ def describe_tile(m: int, n: int, k: int, mode: str = "w8a8-mxfp8", sm_count: in
 
     buf = ctypes.create_string_buffer(256)
     rc = _native.lib().hq_describe_tile(m, n, k, dict(_native.MODE_IDS, **{"w4a8-mxfp4": 3})[mode], sm_count, device, buf, len(buf))
+    if rc != 0:
+        raise RuntimeError(buf.value.decode())
+    return buf.value.decode()
+
+
+def describe_block_tile(m: int, n: int, k: int, num_experts: int = 0, row_scales: bool = False, sm_count: int = -1,
+                        device: int = -1) -> str:
+    """``describe_tile`` for ``block_gemm`` and, with ``num_experts``, ``group_block_gemm``; ``row_scales``: a scale per row
+    on both sides."""
+    import ctypes
+
+    from . import _native
+
+    buf = ctypes.create_string_buffer(256)
+    rc = _native.lib().hq_describe_block_tile(m, n, k, num_experts, int(row_scales), sm_count, device, buf, len(buf))
     if rc != 0:
         raise RuntimeError(buf.value.decode())
     return buf.value.decode()

@@ -63,6 +63,7 @@ SIGNATURES = {
                                                c_char_p, c_size_t]),
     "hq_group_block_gemm": (c_int, [c_void_p] * 6 + [c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_int, c_int, c_int,
                                                      c_void_p, c_char_p, c_size_t]),
+    "hq_describe_block_tile": (c_int, [c_i64, c_i64, c_i64, c_i64, c_int, c_int, c_int, c_char_p, c_size_t]),
     "hq_moe_sort": (c_int, [c_void_p, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                             c_int, c_void_p, c_char_p, c_size_t]),
     "hq_moe_permute": (c_int, [c_void_p, c_i64, c_i64, c_i64, c_i64, c_void_p, c_void_p, c_void_p, c_i64, c_i64, c_int, c_int,

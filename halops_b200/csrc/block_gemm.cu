@@ -1029,6 +1029,27 @@ cudaError_t take_block_gemm_status(uint32_t* status) {
 
 }  // namespace hq
 
+extern "C" int hq_describe_block_tile(int64_t m, int64_t n, int64_t k, int64_t num_experts, int row_scales, int sm_count, int device, char* buf,
+                                      size_t buflen) {
+    if (m < 1 || n < 1 || k < 16 || k % 16 != 0 || num_experts < 0 || num_experts > hq::kMaxExperts || m > INT32_MAX - 128 ||
+        n > INT32_MAX - 256 || k > (int64_t(1) << 30) || (num_experts > 0 && row_scales != 0)) {
+        return hq::fail(buf, buflen, HQ_ERR_INVALID, "No block-128 tile for M=%lld, N=%lld, K=%lld, %lld experts", static_cast<long long>(m),
+                        static_cast<long long>(n), static_cast<long long>(k), static_cast<long long>(num_experts));
+    }
+    const int sms = sm_count > 0 ? sm_count : hq_sm_count(device);
+    hq::BlockProblem g = {};
+    g.rows_a = m, g.n = n, g.k = k, g.experts = std::max<int64_t>(num_experts, 1), g.grouped = num_experts > 0, g.row_scales = row_scales != 0;
+    g.sms = sms > 0 ? sms : 148;
+    g.args.k_tiles = int((k + hq::kBlockK - 1) / hq::kBlockK);
+    const hq::BlockChoice c = hq::choose(g);
+    if (buf != nullptr && buflen > 0) {
+        snprintf(buf, buflen, "[gemm] mode=%s kind=block128%s m=%lld n=%lld k=%lld sm=%d -> %dx%d/%d split=%d", g.grouped ? "experts" : "dense",
+                 g.row_scales ? "-rows" : "", static_cast<long long>(m), static_cast<long long>(n), static_cast<long long>(k), g.sms, hq::kTileM,
+                 c.bn, hq::kBlockK, c.split);
+    }
+    return HQ_OK;
+}
+
 extern "C" int hq_block_gemm(const void* a, const void* b, const float* sfa, const float* sfb, void* out, int out_dtype, int64_t m, int64_t n,
                              int64_t k, int row_scales, int64_t ldo, int sm_count, int use_pdl, int device, void* stream, char* err,
                              size_t errlen) {

@@ -344,6 +344,11 @@ int hq_group_block_gemm(const void* a, const void* b, const float* sfa, const fl
                         void* out, int out_dtype, int64_t num_experts, int64_t m, int64_t n, int64_t k, int64_t ldo,
                         int sm_count, int use_pdl, int device, void* stream, char* err, size_t errlen);
 
+/* The tile that hq_block_gemm (num_experts 0) or hq_group_block_gemm picks for a shape, and the CTAs that share one, as
+ * hq_describe_tile says it for the MX kinds.  Needs no GPU where sm_count is given. */
+int hq_describe_block_tile(int64_t m, int64_t n, int64_t k, int64_t num_experts, int row_scales, int sm_count, int device,
+                           char* buf, size_t buflen);
+
 /*
  * Tokens in the order of the experts that a router gave them, and back (no counterpart in the reference).
  *

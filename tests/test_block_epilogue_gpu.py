@@ -4,7 +4,7 @@ stores, the rings and the buffers must not reach the next.  Tolerances are those
 import pytest
 import torch
 
-from test_block_scale_gpu import BF16, FP16, _assert_product, _ceil, _dequant, _operands, _runs, _values
+from test_block_scale_gpu import BF16, FP16, FP32, _assert_product, _ceil, _dequant, _operands, _runs, _values
 
 pytestmark = pytest.mark.gpu
 
@@ -48,4 +48,47 @@ def test_experts_tiles_after_one_that_sticks_out(hq, n, k):
         at = slice(host[e], host[e + 1])
         if counts[e]:
             _assert_product(first[at], _dequant(a[at], sa[at]), _dequant(b[e], sb[e], (128, 128)), _ceil(k, 128))
+    assert hq.device_status() == 0
+
+
+# width of the tile, rows, columns, K, SMs: every width with several tiles a CTA and the columns of the last that it can have
+MANY = [(64, 1500, 8, 128, 3), (64, 1500, 40, 256, 4), (128, 1500, 72, 16, 3), (128, 2600, 104, 256, 4), (192, 2600, 584, 16, 4),
+        (192, 2600, 616, 128, 4), (192, 1500, 264, 256, 3), (192, 1500, 296, 128, 4), (192, 1500, 136, 16, 4), (192, 1500, 168, 256, 5),
+        (256, 1500, 584, 128, 3), (256, 2600, 616, 16, 3), (256, 1500, 392, 256, 3), (256, 1500, 424, 16, 4), (256, 1500, 200, 128, 4),
+        (256, 1500, 232, 256, 5)]
+
+
+@pytest.mark.parametrize("out", ["bf16", "fp16", "fp32", "odd rows", "behind others"])
+@pytest.mark.parametrize("width,m,n,k,sms", MANY)
+def test_many_tiles_of_every_width(hq, width, m, n, k, sms, out):
+    assert f"128x{width}/128 split=1" in hq.describe_block_tile(m, n, k, sm_count=sms)
+    (a, sa), (b, sb) = _operands(hq, m, n, k, m + n + k)
+    dtype = {"fp16": FP16, "fp32": FP32}.get(out, BF16)
+    ld, skip = {"odd rows": (n + 3, 1), "behind others": (_ceil(n, 8) * 8 + 16, 8)}.get(out, (n, 0))
+    ref, first = (_dequant(a, sa), _dequant(b, sb, (128, 128))), None
+    for _ in range(3):
+        buf = torch.full((m, ld), 7.0, dtype=dtype, device="cuda")
+        y = buf[:, skip : skip + n]
+        hq.block_gemm(a, b, sa, sb, y, sm_count=sms)
+        if first is None:
+            first = buf
+            _assert_product(y, *ref, _ceil(k, 128))
+            assert (buf[:, :skip] == 7).all() and (buf[:, skip + n :] == 7).all()
+        assert torch.equal(buf, first)
+    assert hq.device_status() == 0
+
+
+@pytest.mark.parametrize("m,n,k", [(1500, 1040, 16), (700, 1096, 256), (1500, 264, 400), (1500, 136, 1024)])
+def test_many_tiles_with_a_scale_per_row_on_both_sides(hq, m, n, k):
+    a, sa = hq.block_quant(_values(m, k, m + k))
+    b, sb = hq.block_quant(_values(n, k, n + k + 1))
+    for dtype in (BF16, FP32):
+        first = None
+        for _ in range(3):
+            out = torch.full((m, n), float("nan"), dtype=dtype, device="cuda")
+            hq.block_gemm(a, b, sa, sb, out, sm_count=4)
+            if first is None:
+                first = out
+                _assert_product(out, _dequant(a, sa), _dequant(b, sb), _ceil(k, 128))
+            assert torch.equal(out, first)
     assert hq.device_status() == 0
