@@ -465,7 +465,7 @@ PyObject* moe_sort(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
         Py_RETURN_NONE;
     }
     const int64_t n = ids->numel(), n_rows = (n + std::min<int64_t>(experts, n) * (align - 1)) / align * align;
-    if (n_rows > INT32_MAX) Py_RETURN_NONE;
+    if (n > (int64_t(1) << 31) - 8192 || n_rows > INT32_MAX) Py_RETURN_NONE;
     const void* const p = ids->data_ptr();
     const int dev = ids->get_device();
     void* const st = stream_of(*ids);

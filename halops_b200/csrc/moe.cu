@@ -38,6 +38,7 @@ __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddep
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kMaxExperts = 1024;
+constexpr int64_t kMaxSortPairs = (int64_t(1) << 31) - 8192;  // the kernel's steps past the last pair, and a run's padding, stay below 2^31
 
 template <typename Id>
 __device__ __forceinline__ int expert_of(const Id* ids, int p, int pairs_n, int experts) {
@@ -565,8 +566,10 @@ extern "C" int hq_moe_sort(const void* ids, int ids_bytes, int64_t tokens, int64
     const int rc = hq::check_moe(tokens, topk, n_rows, num_experts, err, errlen);
     if (rc != HQ_OK) return rc;
     if (align < 1 || align > 4096) return fail(err, errlen, HQ_ERR_INVALID, "align must be in [1, 4096], got %lld", static_cast<long long>(align));
+    const int64_t n = tokens * topk;
+    if (n > hq::kMaxSortPairs) return fail(err, errlen, HQ_ERR_INVALID, "at most 2^31 - 8192 pairs, got %lld", static_cast<long long>(n));
     // any ids have to fit: what pads the runs of as many experts as there can be
-    const int64_t n = tokens * topk, need = (n + (n < num_experts ? n : num_experts) * (align - 1)) / align * align;
+    const int64_t need = (n + (n < num_experts ? n : num_experts) * (align - 1)) / align * align;
     if (n_rows < need) {
         return fail(err, errlen, HQ_ERR_INVALID, "%lld rows are needed for %lld pairs, %lld experts and runs on multiples of %lld, got %lld",
                     static_cast<long long>(need), static_cast<long long>(n), static_cast<long long>(num_experts), static_cast<long long>(align),

@@ -28,6 +28,7 @@ __all__ = ["MoeSort", "moe_permute", "moe_permute_backward", "moe_permute_block_
            "moe_unpermute_backward"]
 
 MAX_EXPERTS = 1024
+MAX_PAIRS = 2**31 - 8192
 
 
 class MoeSort(NamedTuple):
@@ -44,7 +45,7 @@ def moe_sort(topk_ids: torch.Tensor, num_experts: int, align: int = 1, use_pdl: 
     """Sorts the pairs (token, slot) of a router's choice by expert; pairs of one expert stay in their order.
 
     Args:
-        topk_ids: [tokens, topk] contiguous CUDA tensor, int32 or int64.  Ids outside of [0, num_experts) are dropped (experts of another
+        topk_ids: [tokens, topk] contiguous CUDA tensor, int32 or int64, at most 2^31 - 8192 pairs.  Ids outside of [0, num_experts) are dropped (experts of another
             device: subtract the first one that is here).  A token may name an expert more than once.
         num_experts: experts here, at most 1024.
         align: every run starts on a multiple of it, at most 4096; the rows that pad a run have no pair.
@@ -62,8 +63,9 @@ def moe_sort(topk_ids: torch.Tensor, num_experts: int, align: int = 1, use_pdl: 
     _check(1 <= num_experts <= MAX_EXPERTS, f"num_experts must be in [1, {MAX_EXPERTS}], got {num_experts}")
     _check(1 <= align <= 4096, f"align must be in [1, 4096], got {align}")
     _check(topk_ids.is_contiguous(), "topk_ids must be contiguous")
-    _on_device(topk_ids.device, topk_ids=topk_ids)
     n = topk_ids.numel()
+    _check(n <= MAX_PAIRS, f"at most 2^31 - 8192 pairs, got {n}")
+    _on_device(topk_ids.device, topk_ids=topk_ids)
     n_rows = (n + min(num_experts, n) * (align - 1)) // align * align
     _check(n_rows < 2**31, f"at most 2^31 - 1 rows, got {n_rows}")
     rows, pairs, offsets, expert_ids = (torch.empty(shape, dtype=torch.int32, device=topk_ids.device)

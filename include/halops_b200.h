@@ -358,7 +358,7 @@ int hq_describe_block_tile(int64_t m, int64_t n, int64_t k, int64_t num_experts,
  *   pairs       [n_rows]           the row's pair, -1 where there is none
  *   offsets     [num_experts + 1]  first row of each run, and the end of the last (padding included)
  *   expert_ids  [n_rows]           the run that a row is in, num_experts - 1 behind the last
- * n_rows is at least floor((p + min(num_experts, p) * (align - 1)) / align) * align for p pairs.
+ * At most 2^31 - 8192 pairs and 2^31 - 1 rows.  n_rows is at least floor((p + min(num_experts, p) * (align - 1)) / align) * align for p pairs.
  */
 int hq_moe_sort(const void* ids, int ids_bytes, int64_t tokens, int64_t topk, int64_t num_experts, int64_t align,
                 int64_t n_rows, int use_pdl, int32_t* rows, int32_t* pairs, int32_t* offsets, int32_t* expert_ids,
