@@ -208,6 +208,19 @@ __device__ __forceinline__ void load_fragments(uint32_t taddr, uint32_t (&r)[16]
         : "memory");
 }
 
+// Scales, which the preceding kernel may still write before pdl_wait: volatile, so that they stay behind it.  (As plain loads, among which
+// the compiler keeps the order of the stores to shared memory, the widest tile spilled.)
+__device__ __forceinline__ float load_scale(const float* p) {
+    float v;
+    asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ float4 load_scales(const float* p) {
+    float4 v;
+    asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+    return v;
+}
+
 // (a, b) += (x, y) * s as one packed instruction.  It needs the issue slots of two scalar ones, but not their operand reads: 128 columns
 // of 8 warps, loads included, take 292 cycles with it and 421 with fmaf.
 __device__ __forceinline__ void add_scaled2(float& a, float& b, uint32_t x, uint32_t y, float s) {
@@ -416,7 +429,7 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
             }
         }
     }
-    // nothing below may run before the preceding kernel's writes are visible
+    // nothing below may run before the preceding kernel's writes are visible (so no load below is one of constant data)
     ptx::pdl_wait();
     if constexpr (kGrouped) {
         if (warp == 0) {
@@ -425,7 +438,7 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
             int* const first_row = tables + kMaxExperts + 8;
             for (int e0 = 0; e0 <= p.experts; e0 += 32) {
                 const int e = e0 + lane;
-                int start = e <= p.experts ? min(max(__ldg(p.offsets + e), 0), p.m) : 0;
+                int start = e <= p.experts ? min(max(p.offsets[e], 0), p.m) : 0;
 #pragma unroll
                 for (int d = 1; d < 32; d *= 2) {
                     const int v = __shfl_up_sync(0xffffffffu, start, d);
@@ -517,11 +530,11 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constan
             const bool wide = p.k_tiles % 4 == 0 && p.wide_scales != 0;
             const auto load4 = [&](const float* q, int k0, float (&v)[kGroupK]) {
                 if (wide && k0 % 4 == 0 && k0 + kGroupK <= k_end) {
-                    const float4 f = __ldg(reinterpret_cast<const float4*>(q + k0));
+                    const float4 f = load_scales(q + k0);
                     v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
                 } else {
 #pragma unroll
-                    for (int i = 0; i < kGroupK; ++i) v[i] = k0 + i < k_end ? __ldg(q + k0 + i) : 0.0f;
+                    for (int i = 0; i < kGroupK; ++i) v[i] = k0 + i < k_end ? load_scale(q + k0 + i) : 0.0f;
                 }
             };
             uint32_t group = 0;

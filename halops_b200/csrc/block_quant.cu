@@ -10,9 +10,10 @@ namespace {
 
 constexpr int kRowThreads = 256;
 
+// (Not ld.global.nc, which is for data that nothing writes while the kernel runs: see block_quant.cuh.)
 __device__ __forceinline__ uint4 load_stream(const void* p) {
     uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
 
@@ -72,7 +73,7 @@ __global__ void __launch_bounds__(kRowThreads) swiglu_block_quant_kernel(const T
     const int lane = threadIdx.x & 31;
     const int64_t task = int64_t(blockIdx.x) * (kRowThreads / 32) + (threadIdx.x >> 5);
     const int64_t row = task / segs;
-    if (row >= m || (row_limit != nullptr && row >= __ldg(row_limit))) return;
+    if (row >= m || (row_limit != nullptr && row >= *row_limit)) return;
     const int c = int(task - row * segs) * 512 + lane * 16;
     const int kb = (k + kQBlock - 1) / kQBlock;
     const T* const src = x + row * ld + c;
@@ -147,11 +148,15 @@ __global__ void __launch_bounds__(kRowThreads) permute_block_quant_kernel(const 
     const BlockScale s = block_scale(magnitude_f32<T>(max8(max(amax16(v), amax16(w)))), true);
     const uint2 lo = codes8<T>(v, s), hi = codes8<T>(w, s);
     if (c >= k) return;
-    for (int j = 0; j < topk; ++j) {
-        const int r = __ldg(rows + token * topk + j);
-        if (r >= 0 && r < n_rows) {
-            *reinterpret_cast<uint4*>(q + int64_t(r) * k + c) = make_uint4(lo.x, lo.y, hi.x, hi.y);
-            if ((threadIdx.x & 7) == 0) sf[int64_t(r) * kb + c / kQBlock] = s.scale;
+    for (int j0 = 0; j0 < topk; j0 += 8) {
+        int r[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[j] = j0 + j < topk ? rows[token * topk + j0 + j] : -1;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (r[j] < 0 || r[j] >= n_rows) continue;
+            *reinterpret_cast<uint4*>(q + int64_t(r[j]) * k + c) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            if ((threadIdx.x & 7) == 0) sf[int64_t(r[j]) * kb + c / kQBlock] = s.scale;
         }
     }
 }

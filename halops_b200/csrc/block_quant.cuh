@@ -26,7 +26,8 @@ constexpr int kQBlock = 128;            // values of a row per scale
 constexpr uint32_t kAmaxFloorBits = 0x2edbe6ffu;  // 1e-10f
 constexpr uint32_t kInfF32 = 0x7f800000u;
 
-// Kernel pointers are not __restrict__: what they point to changes, in the preceding kernel, while this one waits for it.
+// Kernel pointers are not __restrict__ and not read through __ldg: what they point to changes, in the preceding kernel, while this one
+// waits for it, and a load of constant data may be moved to before the wait.
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

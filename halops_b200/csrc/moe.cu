@@ -23,7 +23,8 @@
 namespace hq {
 namespace {
 
-// No kernel pointer here is __restrict__: what it points to changes, in the preceding kernel, while this one waits for it.
+// No kernel pointer here is __restrict__ or read through __ldg: what it points to changes, in the preceding kernel, while this one
+// waits for it, and a load of constant data may be moved to before the wait.
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
@@ -232,12 +233,12 @@ __global__ void __launch_bounds__(kMoveThreads) moe_permute_kernel(const Unit* x
     Unit v[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        if (c + i * kMoveThreads < units) v[i] = __ldg(x + token * ld + c + i * kMoveThreads);
+        if (c + i * kMoveThreads < units) v[i] = x[token * ld + c + i * kMoveThreads];
     }
     for (int j0 = 0; j0 < topk; j0 += 8) {
         int r[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) r[j] = j0 + j < topk ? __ldg(rows + token * topk + j0 + j) : -1;
+        for (int j = 0; j < 8; ++j) r[j] = j0 + j < topk ? rows[token * topk + j0 + j] : -1;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             if (r[j] < 0 || r[j] >= n_rows) continue;
@@ -330,11 +331,11 @@ struct Piece<T, 16> {
     static constexpr int kN = Floats<T>::kN;
     using Vec = typename Floats<T>::Vec;
     Vec v;
-    __device__ __forceinline__ void load(const T* p) { v = __ldg(reinterpret_cast<const Vec*>(p)); }
+    __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const Vec*>(p); }
     // a row that is read once: not kept in L1 (moe_unpermute of 4096 tokens of 4096, 4 of 16: 33.5 -> 27.5 us)
     __device__ __forceinline__ void load_once(const T* p) {
         uint4 u;
-        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p));
+        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p));
         memcpy(&v, &u, 16);
     }
     __device__ __forceinline__ void get(float (&f)[kN]) const { Floats<T>::get(v, f); }
@@ -344,7 +345,7 @@ template <typename T>
 struct Piece<T, 4> {
     static constexpr int kN = 4 / int(sizeof(T));
     uint32_t v;
-    __device__ __forceinline__ void load(const T* p) { v = __ldg(reinterpret_cast<const uint32_t*>(p)); }
+    __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint32_t*>(p); }
     __device__ __forceinline__ void load_once(const T* p) { load(p); }
     __device__ __forceinline__ void get(float (&f)[kN]) const {
         T one[kN];
@@ -396,7 +397,7 @@ __global__ void __launch_bounds__(kMoveThreads) moe_unpermute_kernel(const T* z,
 #pragma unroll
         for (int j = 0; j < kSlots; ++j) {
             int r = -1;
-            if (j0 + j < topk) r = __ldg(rows + token * topk + j0 + j);
+            if (j0 + j < topk) r = rows[token * topk + j0 + j];
             here[j] = r >= 0 && r < n_rows;
             w[j] = 1.0f;
             if (here[j]) {
@@ -404,7 +405,7 @@ __global__ void __launch_bounds__(kMoveThreads) moe_unpermute_kernel(const T* z,
                 for (int q = 0; q < kPer; ++q) {
                     if (c + q * kStep < h) piece[j][q].load_once(z + int64_t(r) * ld + c + q * kStep);
                 }
-                if (weights != nullptr) w[j] = __ldg(weights + token * topk + j0 + j);
+                if (weights != nullptr) w[j] = weights[token * topk + j0 + j];
             }
         }
 #pragma unroll
@@ -453,14 +454,14 @@ __global__ void __launch_bounds__(kMoveThreads) moe_unpermute_backward_kernel(
     }
     const int64_t pair = int64_t(blockIdx.x) * (kMoveThreads / kGroup) + threadIdx.x / kGroup;
     if (pair >= pairs_n) return;  // (whole groups)
-    const int r = __ldg(rows + pair);
+    const int r = rows[pair];
     const bool here = r >= 0 && r < n_rows;
     float dot = 0.0f;
     if (here) {
         const T* const g = gy + pair / topk * ld_g;
         const T* const s = z + int64_t(r) * ld_z;
         T* const to = gz + int64_t(r) * h;
-        const float w = weights != nullptr ? __ldg(weights + pair) : 1.0f;
+        const float w = weights != nullptr ? weights[pair] : 1.0f;
         for (int c0 = (threadIdx.x % kGroup) * P::kN; c0 < h; c0 += kAhead * kStep) {
             P a[kAhead], b[kAhead];
 #pragma unroll
