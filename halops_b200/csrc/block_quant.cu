@@ -64,6 +64,54 @@ __global__ void __launch_bounds__(kRowThreads) block_quant_rows_kernel(const T* 
 // h = gate * sigmoid(gate) * up in float32, quantised from there; gate is the first half of a row, up the second.
 // Rows from *row_limit on (behind the last expert's run) are left alone.
 
+// exp(-a) for a >= 0: 2^t for the rounded t = -a log2(e), corrected by the rest of t, which a second fma gives exactly, so that the error does
+// not grow with a (ex2's 2^-22 and two roundings).  Zero from 87.3 on, below which it would be subnormal.
+__device__ __forceinline__ float exp_minus(float a) {
+    constexpr float kLog2e = 1.44269504f, kLog2eRest = 1.92596299e-8f, kLn2 = 0.693147181f;
+    a = fminf(a, 128.0f);  // (of an infinity the rest would be NaN)
+    const float t = a * -kLog2e;
+    float p;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(t));
+    const float rest = fmaf(a, -kLog2eRest, fmaf(a, -kLog2e, -t));
+    return fmaf(p, rest * kLn2, p);
+}
+
+// gate * sigmoid(gate) from e = exp(-|gate|): nothing overflows, and the divisor is in [1, 2].
+// 16384 x 2 x 2048 takes 33.1 us, with expf and a correctly rounded quotient 42.2, with uncorrected exponentials (3e-6 off at -60, zero below -87.3) 30.2.
+__device__ __forceinline__ float silu(float gate) {
+    const float e = exp_minus(fabsf(gate));
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return (gate < 0.0f ? gate * e : gate) * r;
+}
+
+// Gates below -87: silu leaves the range of normal numbers, while its product with a large `up` may not.  (1 + e is 1 there.)
+constexpr float kFarGate = -87.0f;
+template <typename T>
+constexpr uint32_t kFarBits = 0xc2aeu;  // kFarGate as T: all lower gates, and negative NaNs, have larger bits
+template <>
+constexpr uint32_t kFarBits<__half> = 0xd570u;
+template <bool kFar>
+__device__ __forceinline__ float gated(float gate, float up) {
+    if (kFar && gate < kFarGate) {
+        const float half = exp_minus(-0.5f * gate);
+        return (gate * half) * (up * half);
+    }
+    return silu(gate) * up;
+}
+template <typename T, bool kFar>
+__device__ __forceinline__ void gated16(const uint4 (&gate)[2], const uint4 (&up)[2], float2 (&h)[8]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t gw[4] = {gate[i].x, gate[i].y, gate[i].z, gate[i].w}, uw[4] = {up[i].x, up[i].y, up[i].z, up[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 g = two_floats<T>(gw[j]), u = two_floats<T>(uw[j]);
+            h[i * 4 + j] = make_float2(gated<kFar>(g.x, u.x), gated<kFar>(g.y, u.y));
+        }
+    }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads) swiglu_block_quant_kernel(const T* x, int64_t ld, int64_t m, int k, int segs,
                                                                          const int* row_limit, uint8_t* q,
@@ -85,19 +133,15 @@ __global__ void __launch_bounds__(kRowThreads) swiglu_block_quant_kernel(const T
     }
     float2 h[8];
     uint32_t amax = 0;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const uint32_t gw[4] = {gate[i].x, gate[i].y, gate[i].z, gate[i].w}, uw[4] = {up[i].x, up[i].y, up[i].z, up[i].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 g = two_floats<T>(gw[j]), u = two_floats<T>(uw[j]);
-            float2& o = h[i * 4 + j];
-            // (__fdividef gives 0 for a divisor above 2^126, where the quotient is below 2^-119)
-            o.x = __fdividef(g.x, 1.0f + __expf(-g.x)) * u.x;
-            o.y = __fdividef(g.y, 1.0f + __expf(-g.y)) * u.y;
-            amax = max(amax, max(__float_as_uint(o.x) & 0x7fffffffu, __float_as_uint(o.y) & 0x7fffffffu));
-        }
+    const uint32_t low = __vmaxu2(__vmaxu2(__vmaxu2(gate[0].x, gate[0].y), __vmaxu2(gate[0].z, gate[0].w)),
+                                  __vmaxu2(__vmaxu2(gate[1].x, gate[1].y), __vmaxu2(gate[1].z, gate[1].w)));
+    if (max(low & 0xffffu, low >> 16) <= kFarBits<T>) {
+        gated16<T, false>(gate, up, h);
+    } else {  // (both forms of every value: rare, and as a second pass over the values it cost registers, 16384 x 2 x 2048 39 us)
+        gated16<T, true>(gate, up, h);
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) amax = max(amax, max(__float_as_uint(h[j].x) & 0x7fffffffu, __float_as_uint(h[j].y) & 0x7fffffffu));
     const BlockScale s = block_scale(max8(amax), false);
     if (c < k) {
         uint32_t w[4];

@@ -127,8 +127,9 @@ def swiglu_block_quant(
     output_quant: Optional[torch.Tensor] = None,
     output_sf: Optional[torch.Tensor] = None,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
-    """``silu(gate) * up`` of rows ``[gate | up]``, in float32, quantised in blocks of (1, 128) as ``block_quant`` does: what
-    comes between the two products of a gated MLP or of an expert.
+    """``silu(gate) * up`` of rows ``[gate | up]``, in float32 (off by less than 2^-20 of its value, for any gate whose product is a
+    normal number), quantised in blocks of (1, 128) as ``block_quant`` does: what comes between the two products of a gated MLP or of
+    an expert.
 
     Args:
         input: [m, 2k] CUDA tensor, bfloat16 or float16, ``k`` a multiple of 16; rows may be strided (16-byte aligned).
