@@ -456,7 +456,10 @@ __global__ void __launch_bounds__(kMoveThreads) moe_unpermute_backward_kernel(
     if (pair >= pairs_n) return;  // (whole groups)
     const int r = rows[pair];
     const bool here = r >= 0 && r < n_rows;
-    float dot = 0.0f;
+    // eight sums a thread: one alone would be a chain of h / 32 additions, each of which can lose half a unit of it
+    constexpr int kSums = 8;
+    static_assert(kAhead * P::kN % kSums == 0, "a round of pieces goes round the sums as a whole");
+    float sums[kSums] = {};
     if (here) {
         const T* const g = gy + pair / topk * ld_g;
         const T* const s = z + int64_t(r) * ld_z;
@@ -480,7 +483,7 @@ __global__ void __launch_bounds__(kMoveThreads) moe_unpermute_backward_kernel(
                     float u[P::kN];
                     b[i].get(u);
 #pragma unroll
-                    for (int j = 0; j < P::kN; ++j) dot = fmaf(f[j], u[j], dot);
+                    for (int j = 0; j < P::kN; ++j) sums[(i * P::kN + j) % kSums] = fmaf(f[j], u[j], sums[(i * P::kN + j) % kSums]);
                 }
 #pragma unroll
                 for (int j = 0; j < P::kN; ++j) o[j] = w * f[j];
@@ -489,6 +492,7 @@ __global__ void __launch_bounds__(kMoveThreads) moe_unpermute_backward_kernel(
         }
     }
     if (gw != nullptr) {
+        float dot = ((sums[0] + sums[1]) + (sums[2] + sums[3])) + ((sums[4] + sums[5]) + (sums[6] + sums[7]));
 #pragma unroll
         for (int d = 16; d > 0; d /= 2) dot += __shfl_xor_sync(0xffffffffu, dot, d);
         if constexpr (kGroup > 32) {

@@ -219,7 +219,9 @@ def moe_unpermute_backward(
     Returns:
         ``(grad_input, grad_weights)``: [n_rows, h] with ``weights[pair] * grad_output[token]`` (rows that pad a run are zero, rows
         from ``sort.offsets[-1]`` on are not written), and float32 [tokens, topk] with the products
-        ``<grad_output[token], input[row]>`` (0 for a slot without a row), None where ``weights`` is.
+        ``<grad_output[token], input[row]>`` (0 for a slot without a row), None where ``weights`` is.  A product is summed by a warp, or
+        by 256 threads where there are few pairs, in pieces whose size goes by the rows' alignment: the same call gives the same bits, the
+        same token in a batch of another size may differ in the last ones.
     """
     result = (_native.fast_path or _native.load_fast_path()).moe_unpermute_backward(grad_output, input, sort, weights, use_pdl, grad_input)
     if result is not None:
