@@ -279,7 +279,9 @@ at::Tensor fresh(c10::IntArrayRef shape, at::ScalarType type, c10::Device device
     return at::Tensor(at::detail::empty_cuda(shape, type, device, c10::nullopt));
 }
 
-// Several tensors of one allocation (256-byte aligned), which lives as long as the last of them.
+// Several tensors of one allocation (256-byte aligned), which lives as long as the last of them: for a sort, whose four are of one use (one
+// allocation instead of four saves the host 1.4 of 6.0 us).  Codes and scales have a storage each: in a common one the scales would
+// keep 33 times their bytes, be saved together with the codes, and be gone with them when a caller frees the codes' storage.
 class Together {
     int64_t bytes_ = 0;
     struct Part {
@@ -298,11 +300,6 @@ public:
         bytes_ += (size + 255) / 256 * 256;
     }
     void make(c10::Device device) {
-        if (n_ == 0) return;
-        if (n_ == 1) {
-            *parts_[0].to = fresh(parts_[0].shape, parts_[0].type, device);
-            return;
-        }
         const at::Tensor whole = fresh({bytes_}, at::kByte, device);
         for (int i = 0; i < n_; ++i) {
             const Part& p = parts_[i];
@@ -349,10 +346,8 @@ PyObject* block_quant(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     void* const st = stream_of(*x);
     const c10::Device device = x->device();
     if (unlocked([&](char* err) {
-            Together outputs;
-            if (!q.defined()) outputs.add(&q, qs, at::kFloat8_e4m3fn);
-            if (!sf.defined()) outputs.add(&sf, ss, at::kFloat);
-            outputs.make(device);
+            if (!q.defined()) q = fresh(qs, at::kFloat8_e4m3fn, device);
+            if (!sf.defined()) sf = fresh(ss, at::kFloat, device);
             return g_fn.block_quant(px, ld, batch, type, e, m, k, rows, transpose, pdl, q.data_ptr(), sf.data_ptr(), dev, st, err, kErrLen);
         }) != 0) {
         Py_RETURN_NONE;
@@ -388,10 +383,8 @@ PyObject* swiglu_block_quant(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     void* const st = stream_of(*x);
     const c10::Device device = x->device();
     if (unlocked([&](char* err) {
-            Together outputs;
-            if (!q.defined()) outputs.add(&q, qs, at::kFloat8_e4m3fn);
-            if (!sf.defined()) outputs.add(&sf, ss, at::kFloat);
-            outputs.make(device);
+            if (!q.defined()) q = fresh(qs, at::kFloat8_e4m3fn, device);
+            if (!sf.defined()) sf = fresh(ss, at::kFloat, device);
             return g_fn.swiglu(px, ld, type, m, k, limit, pdl, q.data_ptr(), sf.data_ptr(), dev, st, err, kErrLen);
         }) != 0) {
         Py_RETURN_NONE;
@@ -574,10 +567,8 @@ PyObject* moe_permute_block_quant(PyObject*, PyObject* const* a, Py_ssize_t narg
     void* const st = stream_of(*x);
     const c10::Device device = x->device();
     if (unlocked([&](char* err) {
-            Together outputs;
-            if (!q.defined()) outputs.add(&q, qs, at::kFloat8_e4m3fn);
-            if (!sf.defined()) outputs.add(&sf, ss, at::kFloat);
-            outputs.make(device);
+            if (!q.defined()) q = fresh(qs, at::kFloat8_e4m3fn, device);
+            if (!sf.defined()) sf = fresh(ss, at::kFloat, device);
             return g_fn.moe_permute_quant(px, ld, type, order.tokens, h, order.topk, order.rows, order.pairs, order.offsets, order.experts,
                                           order.n_rows, order.padded, pdl, q.data_ptr(), sf.data_ptr(), dev, st, err, kErrLen);
         }) != 0) {

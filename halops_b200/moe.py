@@ -32,7 +32,8 @@ MAX_PAIRS = 2**31 - 8192
 
 
 class MoeSort(NamedTuple):
-    """Where the pairs (token, slot) of a router's choice are in expert order; int32 CUDA tensors."""
+    """Where the pairs (token, slot) of a router's choice are in expert order; int32 CUDA tensors.  Those of one call may share a storage,
+    which lives as long as the last of them (clone what is kept or saved alone)."""
 
     rows: torch.Tensor  # [tokens, topk]: the pair's row, -1 where its expert is not here
     pairs: torch.Tensor  # [n_rows]: token * topk + slot of the row, -1 where there is none
