@@ -30,7 +30,7 @@ __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddep
 
 // ---------------------------------------------------------------------------- sort
 //
-// A stable counting sort by one cluster of 1 or 8 CTAs.  Every warp has a stretch of the pairs: it counts their experts into a
+// A stable counting sort by one cluster of 1, 8 or 16 CTAs.  Every warp has a stretch of the pairs: it counts their experts into a
 // line of its own in shared memory, the lines are summed over the warps of the CTA and, through distributed shared memory, over the
 // CTAs before this one, and then the warp goes over its stretch again, 32 pairs at a time: a pair's row is its expert's
 // start plus the pairs of that expert before it, counted in the warp's line and, among the 32, by a match of the lanes.  All
@@ -509,15 +509,38 @@ __global__ void __launch_bounds__(kMoveThreads) moe_unpermute_backward_kernel(
 struct SortOptIn {
     std::mutex mu;
     int done[64] = {};
+    int fits[64] = {}, fails[64] = {};  // shared memory a CTA with which a cluster of 16 is known to find room, and not to
 };
+
+// Whether the device, or the part of it that this process has, holds a cluster of 16 CTAs with `bytes` of shared memory each.
+template <typename Id>
+cudaError_t cluster16_fits(SortOptIn& opt, int dev, int bytes, bool* fits) {
+    if (dev >= 0 && dev < 64 && bytes <= opt.fits[dev]) return *fits = true, cudaSuccess;
+    if (dev >= 0 && dev < 64 && opt.fails[dev] != 0 && bytes >= opt.fails[dev]) return *fits = false, cudaSuccess;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(16);
+    cfg.blockDim = dim3(kSortThreads);
+    cfg.dynamicSmemBytes = size_t(bytes);
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 16, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&clusters, moe_sort_kernel<Id>, &cfg);
+    if (e != cudaSuccess) return e;
+    *fits = clusters > 0;
+    if (dev >= 0 && dev < 64) (*fits ? opt.fits : opt.fails)[dev] = bytes;
+    return cudaSuccess;
+}
 
 template <typename Id>
 cudaError_t launch_sort(const void* ids, int pairs_n, int experts, int align, int n_rows, bool pdl, int* rows, int* pairs, int* offsets,
                         int* expert_ids, cudaStream_t stream) {
     static SortOptIn opt;
     // One CTA goes over 128 pairs a warp in 4 steps; from there on 8 CTAs repay the two barriers of their cluster, and 16 (which a kernel
-    // has to opt in to) where there are thousands of pairs for each: 65536 pairs 15.2 -> 11.8 us, 32768 9.6 -> 8.5.
-    const int ctas = pairs_n > 16384 ? 16 : pairs_n > 4096 || n_rows > 16384 ? 8 : 1;
+    // has to opt in to, and for which there has to be room) where there are thousands of pairs for each: 65536 pairs 15.2 -> 11.8 us, 32768 9.6 -> 8.5.
+    int ctas = pairs_n > 16384 ? 16 : pairs_n > 4096 || n_rows > 16384 ? 8 : 1;
     const auto need = [](int e) { return int(sizeof(int)) * (kSortWarps * e + 4 * e + 1); };
     const int bytes = need(experts);
     if (bytes > 40 * 1024 || ctas > 8) {
@@ -530,6 +553,12 @@ cudaError_t launch_sort(const void* ids, int pairs_n, int experts, int align, in
             if (f == cudaSuccess) f = cudaFuncSetAttribute(moe_sort_kernel<Id>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
             if (f != cudaSuccess) return f;
             if (dev >= 0 && dev < 64) opt.done[dev] = 1;
+        }
+        if (ctas > 8) {
+            bool fits = false;
+            const cudaError_t f = cluster16_fits<Id>(opt, dev, bytes, &fits);
+            if (f != cudaSuccess) return f;
+            if (!fits) ctas = 8;
         }
     }
     return launch(moe_sort_kernel<Id>, dim3(ctas), dim3(kSortThreads), size_t(bytes), stream, pdl, unsigned(ctas), static_cast<const Id*>(ids),
