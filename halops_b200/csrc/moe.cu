@@ -711,9 +711,11 @@ extern "C" int hq_moe_unpermute_backward(const void* grad_output, int64_t ld_gra
                ld_input * size % a == 0 && h * size % a == 0;
     };
     const int bytes = fits(16) ? 16 : fits(4) ? 4 : 2;
-    // a warp per pair once they fill the SMs (148 of 16 CTAs' warps), else a CTA
+    // a warp per pair once they fill the SMs (two CTAs of 8 warps each), else a CTA
+    const int sms = hq_sm_count(device);
+    if (sms <= 0) return fail(err, errlen, HQ_ERR_CUDA, "cannot read the SM count of CUDA device %d", device);
     const int64_t n = tokens * topk;
-    const bool warps = n >= 148 * 16;
+    const bool warps = n >= int64_t(sms) * 16;
     const int64_t pair_ctas = warps ? (n + hq::kMoveThreads / 32 - 1) / (hq::kMoveThreads / 32) : n;
     const dim3 grid(unsigned(pair_ctas + (padded != 0 ? num_experts * hq::kPadCtas : 0)));
     const auto go = [&](auto kernel, auto* g) {

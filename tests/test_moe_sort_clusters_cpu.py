@@ -19,3 +19,9 @@ def test_a_cluster_of_16_is_taken_where_there_is_room():
     assert opt_in < ask < go_back < start
     fits = text[text.index("cudaError_t cluster16_fits("): text.index("cudaError_t launch_sort(")]
     assert "cudaOccupancyMaxActiveClusters(&clusters, moe_sort_kernel<Id>, &cfg)" in fits
+
+
+def test_the_number_of_sms_is_the_devices():
+    with open(os.path.join(CSRC, "moe.cu")) as f:
+        text = re.sub(r"//[^\n]*", "", f.read())
+    assert not re.search(r"\b(148|132|144|160)\b", text) and "n >= int64_t(sms) * 16" in text and "sms = hq_sm_count(device)" in text
