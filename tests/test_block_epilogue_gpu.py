@@ -92,3 +92,47 @@ def test_many_tiles_with_a_scale_per_row_on_both_sides(hq, m, n, k):
                 _assert_product(out, _dequant(a, sa), _dequant(b, sb), _ceil(k, 128))
             assert torch.equal(out, first)
     assert hq.device_status() == 0
+
+
+EXPERTS = [1300, 0, 257, 2000, 31, 900]
+
+
+def _assert_rows(y, a, b, k_blocks):
+    """_assert_product, with infinities where a result is beyond FP16 (from 65520 on, half a step above its largest value)."""
+    if y.dtype == FP16:
+        ref, mag = a @ b.t(), a.abs() @ b.abs().t()
+        slack = (130 + k_blocks) * 2.0**-23 * mag
+        beyond = torch.isinf(y)
+        assert (ref.abs()[beyond] >= 65520 - slack[beyond]).all() and (y[beyond] > 0).eq(ref[beyond] > 0).all()
+        assert (ref.abs()[~beyond] <= 65520 + slack[~beyond]).all()
+        assert beyond.float().mean() < 1e-2
+        keep = ~beyond.any(1)
+        y, a = y[keep], a[keep]
+    _assert_product(y, a, b, k_blocks)
+
+
+@pytest.mark.parametrize("out", ["bf16", "fp16", "fp32", "odd rows"])
+@pytest.mark.parametrize("width,n,k,sms", [(64, 40, 256, 3), (128, 72, 16, 3), (128, 120, 256, 4), (192, 776, 16, 3), (192, 264, 256, 3), (192, 312, 128, 4),
+                                           (192, 136, 16, 3), (192, 552, 128, 4), (256, 584, 256, 3), (256, 632, 128, 4), (256, 392, 16, 3),
+                                           (256, 440, 128, 3), (256, 712, 16, 5), (256, 488, 256, 4)])
+def test_many_tiles_of_experts(hq, width, n, k, sms, out):
+    offsets, rows = _runs(EXPERTS)
+    assert f"128x{width}/128" in hq.describe_block_tile(rows, n, k, len(EXPERTS), sm_count=sms)
+    a, sa = hq.block_quant(_values(rows, k, n))
+    b, sb = hq.block_quant(_values(len(EXPERTS) * n, k, n + 1).view(len(EXPERTS), n, k), (128, 128))
+    dtype = {"fp16": FP16, "fp32": FP32}.get(out, BF16)
+    ld, skip = (n + 3, 1) if out == "odd rows" else (n, 0)
+    first, host = None, offsets.tolist()
+    for _ in range(3):
+        buf = torch.full((rows, ld), 7.0, dtype=dtype, device="cuda")
+        y = buf[:, skip : skip + n]
+        hq.group_block_gemm(a, b, sa, sb, offsets, y, sm_count=sms)
+        if first is None:
+            first = buf
+            for e, count in enumerate(EXPERTS):
+                at = slice(host[e], host[e + 1])
+                if count:
+                    _assert_rows(y[at], _dequant(a[at], sa[at]), _dequant(b[e], sb[e], (128, 128)), _ceil(k, 128))
+            assert (buf[:, :skip] == 7).all() and (buf[:, skip + n :] == 7).all()
+        assert torch.equal(buf, first)
+    assert hq.device_status() == 0
