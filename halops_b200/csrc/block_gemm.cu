@@ -17,7 +17,8 @@
 // What bounds it.  A k-tile of 256 columns takes 850 to 870 cycles, 512 of them MMAs (ncu: the tensor pipe busy for 52 % of 4096 x 7168 x 2048, L2
 // and the way from it for a third, issue slots for 39 %).  Without the promotion's products it takes 640 to 670; the rest is the round of
 // the promotion (287 cycles of loads and 260 of products, one after the other in warps that wait together).  Large problems run
-// at the power cap besides: 8192 x 8192 x 8192 takes 545 to 605 us at 1.38 GHz and 990 W (the MXFP8 kernel 432 at 1.17).  Measured and left:
+// at the power cap besides: 8192 x 8192 x 8192 takes 545 to 605 us at 1.38 GHz and 990 W (the MXFP8 kernel 432 at 1.17), 458 in a burst of a few
+// milliseconds.  Measured and left:
 // 16 promotion warps on 256 columns (registers spill; 595 us against 540), double-buffered loads (648), half of B's bytes, as a CTA pair
 // would load (518, without what a pair's remote signals would add).
 //
@@ -918,11 +919,18 @@ struct BlockChoice {
     int bn, split;
 };
 
-// The least time by figures of the three tiles, GEMM alone.  A k-tile takes `alone` microseconds with few CTAs running and `full` with all
-// (then the CTAs share L2 and power): 16 x 4096 x 7168 on 64 columns 11.8 us, 128 x 4096 x 16384 24.9, 8192 x 8192 x 8192 786 (128
-// columns: 14.6, 28.6, 579; 256: -, -, 484 to 558); `tile` is what a tile's end costs, and a launch is 3.  With a CTA's share of
-// K in `split` CTAs of a cluster: 2.2 more for its barriers and the exchange (16 x 4096 x 7168 on 128 columns 15.4 us whole, 9.3
-// in four; 8 x 1024 x 4096 11.2 whole, 6.1 in eight; 1 x 7168 x 2048 6.7 whole, 7.3 in two).
+// The least time by figures of the four tiles, GEMM alone.  A k-tile takes `alone` microseconds with few CTAs running and `full` with all
+// (then the CTAs share L2 and power); `tile` is what a tile's end costs, and a launch is 3.  Measured for 64, 128, 192, 256 columns:
+//   8 tiles, K from 4096 to 16384                0.139  0.187  0.311  0.396 a k-tile
+//   8192 x 8192 x 8192 in a burst                0.179  0.270  0.400  0.511 a k-tile; 640, 484, 486, 458 us
+//   the same at the power cap                    -      0.336  0.492  0.638 a k-tile; -, 602, 598, 572 us
+//   9472 rows by 2 and by 20 widths, K = 256     0.47   0.71   0.79   1.32 a tile beside its k-tiles
+// The table stands between the burst and the cap.  Of 20 shapes from 16 x 4096 x 7168 to 8192 x 8192 x 8192, each on all four widths, the chosen one
+// was the fastest on 18 and within 3.5 % on the others (4736 x 768 x 4096: 22.3, 21.2, 17.4, 21.0 us; 2048 x 1024 x 2048: 9.2, 7.4, 9.8, 11.1;
+// 1000 x 4104 x 4112: 48.4, 34.7, 42.0, 27.4).  Scales per row on both sides have dearer k-tiles than the table's: 128 columns are chosen and
+// right for 7168 x 2048 x 4096 (109 us, 124 on 64), but 64 are faster where K is short (1024 x 2048 x 256 5.6 us, 7.1 chosen).
+// With a CTA's share of K in `split` CTAs of a cluster: 2.2 more for its barriers and the exchange (16 x 4096 x 7168 on 128 columns 13.1 us whole,
+// 9.8 in two, 8.4 in four; 8 x 1024 x 4096 8.5 whole, 5.5 in eight; 1 x 7168 x 2048 5.9 whole, 6.4 in two).
 BlockChoice choose(const BlockProblem& g) {
     struct Cost {
         int bn;

@@ -7,7 +7,8 @@
 // and so has amax; a midpoint has 5 at most and 448 = 7 * 64.  x * 448 / amax therefore either is a midpoint or differs from
 // it by 2^-16 of its value at least, and rounding the product to a multiple of 8 units of its last place (2^-20 of the
 // value at most) puts it back on the midpoint where it belongs there and moves nothing else across: the codes are those of the
-// exact quotient.
+// exact quotient.  (Below the floor amax has 24 bits, and no quotient is a midpoint; that none is near enough to one to be moved onto
+// it was tried for all 11996 bf16 magnitudes there.)
 // A NaN or an infinity in a block makes its scale NaN or infinite (as maximum of the bit patterns, where NaN is
 // above infinity and infinity above the rest), so that every product with the block is NaN.
 #pragma once

@@ -186,10 +186,12 @@ def block_gemm(
     sm_count: int = -1,
     use_pdl: bool = True,
 ) -> None:
-    """``output = (input * sfa) @ (weight * sfb)^T``, summed in float32 and rounded once.
+    """``output = (input * sfa) @ (weight * sfb)^T``, summed in float32 and rounded once.  The two scales of a block are multiplied in float32 (with
+    a scale per row on both sides one after the other onto the sums): their product has to be a finite, normal number, as those of
+    ``block_quant`` are for values whose magnitudes multiply to less than 1e43.
 
     Args:
-        input: [M, K] float8_e4m3fn, ``K`` a multiple of 16.
+        input: [M, K] float8_e4m3fn, ``K`` a positive multiple of 16.
         weight: [N, K] float8_e4m3fn.
         sfa: float32 [M, ceil(K/128)], as ``block_quant(x)`` returns it.
         sfb: float32 [ceil(N/128), ceil(K/128)] (``block_quant(w, (128, 128))``) or [N, ceil(K/128)], a scale per row of
